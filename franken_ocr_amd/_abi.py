@@ -112,6 +112,17 @@ _SIGS: dict[str, list] = {
     "focr_hip_rswa_get_state": [_P, _SZ, _P, _P, _P],
     "focr_hip_rswa_set_state": [_P, _SZ, C.c_uint32, C.c_uint32],
     "focr_hip_rswa_regions": [_P, _SZ, _P, _P, _P, _P],
+    "focr_hip_paged_create": [_P, _SZ, _SZ, _SZ, _SZ, _I32, _P, _P, _P],
+    "focr_hip_paged_free": [_P],
+    "focr_hip_paged_regions": [_P, _P, _P],
+    "focr_hip_paged_write": [_P, _P, _P, _P, _SZ, _SZ, _P, _P, _P, _SZ, _SZ, _I32],
+    "focr_hip_paged_attention": [_P, _P, _P, _SZ, _SZ, _P, _SZ, _SZ, _P, _SZ, _P, _SZ, _F32, _P, _SZ, _P, _SZ, _I32],
+    "focr_hip_paged_step": [_P, _P, _P, _SZ, _SZ, _P, _P, _SZ, _P, _SZ, _SZ, _P, _SZ, _P, _SZ, _F32, _P, _SZ, _P, _SZ,
+                            _I32, _I32],
+    "focr_hip_paged_evict": [_P, _P, _P, _SZ, _SZ, _P, _SZ, _P, _SZ, _SZ, _SZ, _SZ, _P, _SZ, _P, _P, _SZ, _P, _I32],
+    "focr_hip_beam_select": [_P, _P, _SZ, _SZ, _SZ, _SZ, _P, _P, C.c_uint32, _P, _SZ, _P, _SZ, _SZ, _P, _SZ, _P, _P, _P,
+                             _P, _I32],
+    "focr_hip_beam_reorder": [_P, _SZ, _SZ, _P, _P, _P, _SZ, _P, _I32, _P, _SZ, _P, _SZ, _P, _P, _SZ, _I32],
     "focr_hip_focrq_open": [C.c_char_p, _P],
     "focr_hip_focrq_from_bytes": [_P, _SZ, _P],
     "focr_hip_focrq_close": [_P],

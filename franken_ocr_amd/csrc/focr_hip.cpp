@@ -98,9 +98,17 @@ void* focr_hip_ctx::scratch_get(int slot, size_t bytes) {
     if (b.cap >= bytes) return b.p;
     if (b.p) {
         hipStreamSynchronize(stream);
-        hipFree(b.p);
+        if (!b.captured) {
+            hipFree(b.p);
+        } else {
+            try {
+                retired.push_back(b.p);
+            } catch (const std::bad_alloc&) {  // stays allocated, unlisted
+            }
+        }
         b.p = nullptr;
         b.cap = 0;
+        b.captured = false;
     }
     size_t cap = std::max(bytes, static_cast<size_t>(4096));
     cap = (cap + 255) & ~static_cast<size_t>(255);
@@ -111,6 +119,23 @@ void* focr_hip_ctx::scratch_get(int slot, size_t bytes) {
         return nullptr;
     }
     b.cap = cap;
+    return b.p;
+}
+
+bool focr_hip_ctx::captures() const {
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    return hipStreamIsCapturing(stream, &cap) != hipSuccess || cap != hipStreamCaptureStatusNone;
+}
+
+void* focr_hip_ctx::scratch_get_capturable(int slot, size_t bytes, const char* who) {
+    if (!captures()) return scratch_get(slot, bytes);
+    Buf& b = scratch[slot];
+    if (!b.p || b.cap < bytes) {
+        fail(FOCR_HIP_E_STATE, fmt("%s: %zu bytes of scratch are not there yet and a capture cannot allocate them; make "
+                                   "the same call once before the capture", who, bytes));
+        return nullptr;
+    }
+    b.captured = true;
     return b.p;
 }
 
@@ -188,6 +213,7 @@ int32_t focr_hip_ctx_destroy(focr_hip_ctx* ctx) {
     hipStreamSynchronize(ctx->stream);
     for (auto& b : ctx->scratch)
         if (b.p) hipFree(b.p);
+    for (void* p : ctx->retired) hipFree(p);
     for (auto& p : ctx->pending) {
         hipEventDestroy(p.start);
         hipEventDestroy(p.stop);

@@ -55,6 +55,10 @@ enum ScratchSlot : int {
     kScrLayer,  // decoder layer step intermediates
     kScrAttn,   // prefill attention key-range partials
     kScrDec,    // decode step: the final-normed rows
+    kScrPaged,  // paged attention: split partials, scores
+    kScrEvict,  // eviction: selection tables, kept slots
+    kScrBeam,   // beam selection: per-chunk candidates and sums
+    kScrCheck,  // checks of paged / beam arguments: the first fault found
     kScrCount
 };
 
@@ -105,7 +109,9 @@ struct focr_hip_ctx {
     struct Buf {
         void* p = nullptr;
         size_t cap = 0;
+        bool captured = false;  // part of a captured graph: never freed before the context
     } scratch[focr::kScrCount];
+    std::vector<void*> retired;  // outgrown buffers that captured graphs still use
     // this device's static scratch (focr::static_scratch_init), or null with
     // the error that kept it from resolving
     void* static_scratch = nullptr;
@@ -121,6 +127,11 @@ struct focr_hip_ctx {
 
     // Grow-only scratch. Returns nullptr (and sets the error) on failure.
     void* scratch_get(int slot, size_t bytes);
+    // The same for entry points whose calls may be captured: while the stream
+    // captures, a buffer that is too small is not grown (null, with the error
+    // set), and one that is given is kept until the context goes.
+    void* scratch_get_capturable(int slot, size_t bytes, const char* who);
+    bool captures() const;
     // Make current the device this context lives on.
     hipError_t bind() const { return hipSetDevice(device); }
     hipEvent_t take_event();
@@ -217,6 +228,21 @@ struct focr_hip_rswa {
     float* ref_v(size_t s) const;
     float* ring_k(size_t s) const;
     float* ring_v(size_t s) const;
+};
+
+// Pools of pages of one layer's keys and values, [n_pages][n_kv_heads]
+// [page_size][head_dim] each, and their geometry. Page tables and lengths are
+// the caller's device arrays, given with every call.
+struct focr_hip_paged {
+    focr_hip_ctx* ctx = nullptr;
+    size_t n_pages = 0, n_kv_heads = 0, head_dim = 0;
+    int page_shift = 0;  // page_size = 1 << page_shift
+    int32_t dtype = 0;   // FOCR_HIP_DT_F32 / F16 / BF16
+    void* k = nullptr;
+    void* v = nullptr;
+    bool owned = false;
+    size_t esize() const { return dtype == FOCR_HIP_DT_F32 ? 4 : 2; }
+    size_t page_bytes() const { return (n_kv_heads * head_dim * esize()) << page_shift; }
 };
 
 namespace focr {
@@ -669,5 +695,117 @@ hipError_t launch_rswa_attention(hipStream_t s, const focr_hip_rswa* c, size_t s
                                  const RswaStepArgs& a, const float* q, float* out,
                                  float* partials, focr_hip_ctx* ctx,
                                  const float* k_steps = nullptr, const float* v_steps = nullptr);
+
+// k_paged.hip — the paged cache. Row r of the tables is sequence r's pages.
+constexpr uint32_t kPagedNone = 0xFFFFFFFFu;  // lens[s]: no sequence in this row
+constexpr int kPagedChunkMax = 2048;          // keys of one split
+constexpr int kPagedChunkUnit = 64;           // splits are whole multiples of this
+struct PagedTables {
+    const uint32_t* tables;  // [n_seqs][max_pages]
+    const uint32_t* lens;    // [n_seqs]
+    int n_seqs;
+    size_t max_pages;
+    uint32_t max_len;  // what a length may be at most (<= max_pages * page_size)
+};
+struct PagedAttend {
+    PagedTables t;
+    const uint32_t* prefix;  // nullable
+    uint32_t window;         // 0: every key is seen
+    const float* q;
+    size_t ldq;
+    int group;  // query heads to a key head
+    float scale;
+    const float* k_steps;  // a step's new rows (nullable: attention alone)
+    const float* v_steps;
+    size_t ldkv;
+    uint32_t* lens_advance;  // the lengths again where the step counts them up (nullable)
+    float* out;
+    size_t ldo;
+    float* weights;  // [n_seqs][n_kv_heads][ldw], nullable
+    size_t ldw;
+    int nsplit;
+    // workspace
+    uint4* seen;     // [n_seqs]
+    float2* part_ml; // [n_seqs][n_heads][nsplit]
+    float* part_acc; // [n_seqs][n_heads][nsplit][head_dim]
+    float* scores;   // [n_seqs][n_heads][score_ld] with weights
+    size_t score_ld;
+};
+int paged_pick_splits(size_t n_seqs, size_t kv_heads, int group, uint32_t max_seen, int cu_count);
+hipError_t launch_paged_attend(hipStream_t s, const focr_hip_paged* c, const PagedAttend& a, focr_hip_ctx* ctx);
+hipError_t launch_paged_write(hipStream_t s, const focr_hip_paged* c, const float* k, const float* v, size_t ld,
+                              size_t rows, const uint32_t* seq, const uint32_t* pos, const uint32_t* tables,
+                              int n_seqs, size_t max_pages);
+// Eviction: of every (sequence, kv head), which slots stay; then their rows
+// into the pages of dst_tables.
+struct PagedEvict {
+    PagedTables t;
+    const float* weights;  // [n_seqs][n_kv_heads][ldw]
+    size_t ldw;
+    uint32_t budget, sinks, recent;
+    const uint32_t* dst_tables;  // [n_seqs][dst_max_pages]
+    size_t dst_max_pages;
+    uint32_t* dst_lens;
+    float* dst_weights;  // [n_seqs][n_kv_heads][dst_ldw]
+    size_t dst_ldw;
+    uint32_t* kept;  // [n_seqs][n_kv_heads][budget]
+};
+hipError_t launch_paged_evict(hipStream_t s, const focr_hip_paged* c, const PagedEvict& a, focr_hip_ctx* ctx);
+// Checks for calls that ask for them: err[0] = 0 where all is well, else
+// (row << 8 | code) + 1 of the first fault.
+enum PagedFault : int { kFaultLen = 1, kFaultPage = 2, kFaultSeq = 3, kFaultDstPage = 4, kFaultDstShared = 5,
+                        kFaultParent = 6, kFaultGroupLen = 7, kFaultTail = 8, kFaultHistory = 9 };
+hipError_t launch_paged_check(hipStream_t s, const focr_hip_paged* c, const PagedTables& t, uint32_t add,
+                              const uint32_t* prefix, uint32_t window, unsigned long long* err);
+hipError_t launch_paged_check_rows(hipStream_t s, const focr_hip_paged* c, size_t rows, const uint32_t* seq,
+                                   const uint32_t* pos, const uint32_t* tables, int n_seqs, size_t max_pages,
+                                   unsigned long long* err);
+// marks: n_pages bits of scratch
+hipError_t launch_paged_check_dst(hipStream_t s, const focr_hip_paged* c, const PagedEvict& a, uint32_t* marks,
+                                  unsigned long long* err);
+hipError_t launch_clear_words(hipStream_t s, uint32_t* p, size_t n);
+
+// k_beam.hip — beam search: selection over beams and vocabulary, and the
+// states of the chosen beams put where their slots are.
+constexpr int kBeamMax = 32;
+struct BeamSelect {
+    const float* logits;  // [groups * beams][ld]
+    size_t ld;
+    int groups, beams, vocab;
+    const float* scores;
+    const uint8_t* done;  // nullable
+    uint32_t eos;
+    const uint32_t* ban_bits;  // nullable, [groups * beams][ban_words]
+    int ban_words;
+    uint32_t* parents;
+    uint32_t* tokens;
+    float* new_scores;
+    uint8_t* new_done;  // nullable
+    int nparts;         // chunks of a row
+    void* part;         // beam_part_bytes()
+};
+int beam_parts(int vocab);  // chunks of a row
+size_t beam_part_bytes(int rows, int beams, int nparts);
+hipError_t launch_beam_select(hipStream_t s, const BeamSelect& a, focr_hip_ctx* ctx);
+struct BeamReorder {
+    int groups, beams;
+    const uint32_t* parents;
+    const uint32_t* tokens;  // nullable
+    uint32_t* history;       // nullable
+    size_t cap;
+    uint32_t* history_len;
+    int advance;
+    uint32_t* tables;  // nullable
+    size_t max_pages;
+    const uint32_t* lens;
+    int page_shift;
+    int permute;  // the tables follow the parents
+};
+// One launch: the histories and tables, the pages in progress of the caches
+// and the first ring_rows slots of the rings.
+hipError_t launch_beam_reorder(hipStream_t s, const BeamReorder& a, const focr_hip_paged* const* caches,
+                               size_t n_caches, const focr_hip_rswa* const* rings, size_t n_rings,
+                               uint32_t ring_rows);
+hipError_t launch_beam_check(hipStream_t s, const BeamReorder& a, unsigned long long* err);
 
 }  // namespace focr

@@ -1,0 +1,780 @@
+// k_paged.hip — one new token over a paged key-value cache: the write of its
+// rows, the attention split over the cache's length, the join of the splits,
+// the attention weight each key gathers, and eviction by that weight.
+//
+// Layout in HBM: K and V pools [n_pages][n_kv_heads][page_size][head_dim], so
+// the slots of one (page, head) are contiguous. Key j of sequence s is slot
+// j % page_size of page tables[s][j / page_size]. A call sees of n keys all,
+// or (window w > 0) the first p = min(prefix, n) and the last w:
+//   s_j = scale q.k_j, P_j = exp(s_j - max s) / sum exp, out = sum_j P_j v_j.
+// Scores are kept times log2 e, so that the exponential is the hardware's
+// exp2. Dots, the running maximum and sum and the outputs are f32; the only
+// rounding to fewer bits is a written row's to the cache's type.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "focr_internal.hpp"
+#include "k_common.hpp"
+#include "k_paged_index.hpp"
+
+namespace focr {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+PoolGeom geom_of(const focr_hip_paged* c) {
+    return PoolGeom{c->k, c->v, static_cast<uint32_t>(c->n_pages), c->page_shift,
+                    static_cast<uint32_t>(c->n_kv_heads)};
+}
+
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+// 16 bytes of a row as floats, and back (round to nearest, ties to even).
+template <typename T>
+struct Row16;
+template <>
+struct Row16<float> {
+    static constexpr int N = 4;
+    static __device__ __forceinline__ void load(const u4& w, float* f) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(w[i]);
+    }
+    static __device__ __forceinline__ u4 pack(const float* f) {
+        u4 w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(f[i]);
+        return w;
+    }
+};
+template <>
+struct Row16<__bf16> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ void load(const u4& w, float* f) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f[2 * i] = __uint_as_float(w[i] << 16);
+            f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+    }
+    static __device__ __forceinline__ u4 pack(const float* f) {
+        u4 w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t lo = __builtin_bit_cast(uint16_t, static_cast<__bf16>(f[2 * i]));
+            const uint32_t hi = __builtin_bit_cast(uint16_t, static_cast<__bf16>(f[2 * i + 1]));
+            w[i] = lo | (hi << 16);
+        }
+        return w;
+    }
+};
+template <>
+struct Row16<_Float16> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ void load(const u4& w, float* f) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f[2 * i] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w[i] & 0xFFFFu)));
+            f[2 * i + 1] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w[i] >> 16)));
+        }
+    }
+    static __device__ __forceinline__ u4 pack(const float* f) {
+        u4 w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t lo = __builtin_bit_cast(uint16_t, static_cast<_Float16>(f[2 * i]));
+            const uint32_t hi = __builtin_bit_cast(uint16_t, static_cast<_Float16>(f[2 * i + 1]));
+            w[i] = lo | (hi << 16);
+        }
+        return w;
+    }
+};
+
+// Lane l's value with lane (l ^ M)'s: within a 16-lane row by DPP, across rows
+// by v_permlane16_swap / v_permlane32_swap (VALU; a shuffle goes through LDS).
+template <int M, typename Op>
+__device__ __forceinline__ float xor_fold(float v, Op op) {
+    if constexpr (M == 1) return op(v, __int_as_float(dpp_mov<0xB1>(__float_as_int(v))));
+    if constexpr (M == 2) return op(v, __int_as_float(dpp_mov<0x4E>(__float_as_int(v))));
+    if constexpr (M == 4) {  // after 1 and 2 every quad is uniform: the half row's mirror is the other quad
+        return op(v, __int_as_float(dpp_mov<0x141>(__float_as_int(v))));
+    }
+    if constexpr (M == 8) return op(v, __int_as_float(dpp_mov<0x128>(__float_as_int(v))));  // row_ror:8
+    if constexpr (M == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        return op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    }
+    if constexpr (M == 32) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        return op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    }
+    return v;
+}
+
+struct Sum {
+    __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
+};
+struct Max {
+    __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+};
+
+// Over the lanes that differ in the bits [A, B) of their number (powers of
+// two); every lane gets the result. A = 1 or A >= 8.
+template <int A, int B, typename Op>
+__device__ __forceinline__ float fold_lanes(float v, Op op) {
+    if constexpr (A < B) {
+        v = xor_fold<A>(v, op);
+        return fold_lanes<2 * A, B>(v, op);
+    }
+    return v;
+}
+
+// One split of one key head's keys, for GT of its query heads. Grid (split,
+// key head x head tile, sequence), 4 waves. Every wave takes tiles of its own:
+// C lanes hold a key's row (16 bytes each), 64 / C keys to a load
+// instruction, U of those for K and U for V in flight at once; a lane keeps
+// the same key's K and V, so the probabilities never leave their lanes, and
+// there is no barrier until the four waves' maxima, sums and outputs are
+// joined at the end.
+template <typename T, int D, int GT, int U>
+__global__ __launch_bounds__(256) void paged_attend_kernel(PoolGeom g, PagedAttend a) {
+    constexpr int E = Row16<T>::N;
+    constexpr int C = D / E;
+    constexpr int R = 64 / C;
+    constexpr int TILE = U * R;
+    static_assert(kPagedChunkUnit % TILE == 0 || TILE % kPagedChunkUnit == 0, "a padded split stays in s_row");
+    __shared__ uint32_t s_row[kPagedChunkMax];
+    __shared__ float s_acc[4][GT][D];
+    __shared__ float2 s_ml[4][GT];
+    const int z = blockIdx.x;
+    const int tiles = (a.group + GT - 1) / GT;
+    const int hk = blockIdx.y / tiles;
+    const int g0 = (blockIdx.y - hk * tiles) * GT;  // the first of this block's query heads in the group
+    const int s = blockIdx.z;
+    const Seen e = seen_of(a.t, a.prefix, a.window, a.k_steps != nullptr, s);
+    if (z == 0 && blockIdx.y == 0 && threadIdx.x == 0)
+        a.seen[s] = make_uint4(e.none ? kPagedNone : e.nvis, e.p, e.shift, e.own ? 1u : 0u);
+    if (e.none) return;
+    const uint32_t chunk = split_keys(e.nvis, a.nsplit);
+    const uint32_t b0 = static_cast<uint32_t>(z) * chunk;
+    if (b0 >= e.nvis) return;
+    const int cnt = static_cast<int>(min(chunk, e.nvis - b0));
+    const int padded = (cnt + TILE - 1) / TILE * TILE;
+    for (int j = threadIdx.x; j < padded; j += 256) {
+        const uint32_t at = b0 + j;
+        s_row[j] = j < cnt ? row_of(a.t, g, s, hk, at < e.p ? at : at + e.shift) : kBadRow;
+    }
+    const int wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63;
+    const int cl = lane % C;  // which 16 bytes of a row
+    const int r = lane / C;   // which key of a load instruction
+    float q[GT][E];
+    const float qscale = a.scale * kLog2e;
+#pragma unroll
+    for (int i = 0; i < GT; ++i) {
+        const float* qr = a.q + static_cast<size_t>(s) * a.ldq + (static_cast<size_t>(hk) * a.group + g0 + i) * D + cl * E;
+#pragma unroll
+        for (int j = 0; j < E; ++j) q[i][j] = g0 + i < a.group ? qr[j] * qscale : 0.0f;
+    }
+    // the step's own row is the last key seen
+    const int own = e.own && e.nvis - 1 - b0 < static_cast<uint32_t>(cnt) ? static_cast<int>(e.nvis - 1 - b0) : -1;
+    float m[GT], l[GT], acc[GT][E];
+#pragma unroll
+    for (int i = 0; i < GT; ++i) {
+        m[i] = -INFINITY;
+        l[i] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < E; ++j) acc[i][j] = 0.0f;
+    }
+    __syncthreads();
+    const u4* kp = static_cast<const u4*>(g.k) + cl;
+    const u4* vp = static_cast<const u4*>(g.v) + cl;
+    const size_t head0 = static_cast<size_t>(hk) * a.group + g0;
+    const size_t n_heads = static_cast<size_t>(g.kv_heads) * a.group;
+    for (int t0 = wave * TILE; t0 < cnt; t0 += 4 * TILE) {
+        uint32_t row[U];
+        bool all = true;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            row[u] = s_row[t0 + u * R + r];
+            all = all && row[u] != kBadRow;
+        }
+        u4 kw[U], vw[U];
+        if (__all(all)) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) kw[u] = kp[static_cast<size_t>(row[u]) * C];
+#pragma unroll
+            for (int u = 0; u < U; ++u) vw[u] = vp[static_cast<size_t>(row[u]) * C];
+        } else {  // slots that hold no key are not read: what lies there may be NaN
+#pragma unroll
+            for (int u = 0; u < U; ++u) kw[u] = row[u] != kBadRow ? kp[static_cast<size_t>(row[u]) * C] : u4{0, 0, 0, 0};
+#pragma unroll
+            for (int u = 0; u < U; ++u) vw[u] = row[u] != kBadRow ? vp[static_cast<size_t>(row[u]) * C] : u4{0, 0, 0, 0};
+        }
+        if (own >= t0 && own < t0 + TILE) {  // the step's row comes from the call and goes to its page
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (t0 + u * R + r == own && row[u] != kBadRow) {
+                    const size_t at = static_cast<size_t>(s) * a.ldkv + static_cast<size_t>(hk) * D + cl * E;
+                    float f[E];
+#pragma unroll
+                    for (int j = 0; j < E; ++j) f[j] = a.k_steps[at + j];
+                    kw[u] = Row16<T>::pack(f);
+#pragma unroll
+                    for (int j = 0; j < E; ++j) f[j] = a.v_steps[at + j];
+                    vw[u] = Row16<T>::pack(f);
+                    if (g0 == 0) {
+                        static_cast<u4*>(g.k)[static_cast<size_t>(row[u]) * C + cl] = kw[u];
+                        static_cast<u4*>(g.v)[static_cast<size_t>(row[u]) * C + cl] = vw[u];
+                    }
+                }
+            }
+        }
+        float sc[U][GT];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float f[E];
+            Row16<T>::load(kw[u], f);
+#pragma unroll
+            for (int i = 0; i < GT; ++i) {
+                float d = f[0] * q[i][0];
+#pragma unroll
+                for (int j = 1; j < E; ++j) d = fmaf(f[j], q[i][j], d);
+                d = fold_lanes<1, C>(d, Sum());
+                sc[u][i] = row[u] != kBadRow ? d : -INFINITY;
+            }
+        }
+        if (a.scores) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int j = t0 + u * R + r;
+                if (cl == 0 && j < cnt)
+#pragma unroll
+                    for (int i = 0; i < GT; ++i)
+                        if (g0 + i < a.group)
+                            a.scores[(static_cast<size_t>(s) * n_heads + head0 + i) * a.score_ld + b0 + j] = sc[u][i];
+            }
+        }
+        float safe[GT];
+#pragma unroll
+        for (int i = 0; i < GT; ++i) {
+            float mx = sc[0][i];
+#pragma unroll
+            for (int u = 1; u < U; ++u) mx = fmaxf(mx, sc[u][i]);
+            mx = fmaxf(fold_lanes<C, 64>(mx, Max()), m[i]);
+            safe[i] = mx == -INFINITY ? 0.0f : mx;  // no key yet: every exponential is 0, not NaN
+            const float corr = __builtin_amdgcn_exp2f(m[i] - safe[i]);
+            m[i] = mx;
+            l[i] *= corr;
+#pragma unroll
+            for (int j = 0; j < E; ++j) acc[i][j] *= corr;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float f[E];
+            Row16<T>::load(vw[u], f);
+#pragma unroll
+            for (int i = 0; i < GT; ++i) {
+                const float p = __builtin_amdgcn_exp2f(sc[u][i] - safe[i]);
+                l[i] += p;
+#pragma unroll
+                for (int j = 0; j < E; ++j) acc[i][j] = fmaf(p, f[j], acc[i][j]);
+            }
+        }
+    }
+    // the R keys of a wave's lanes, then the waves
+#pragma unroll
+    for (int i = 0; i < GT; ++i) {
+        l[i] = fold_lanes<C, 64>(l[i], Sum());
+#pragma unroll
+        for (int j = 0; j < E; ++j) acc[i][j] = fold_lanes<C, 64>(acc[i][j], Sum());
+        if (lane == 0) s_ml[wave][i] = make_float2(m[i], l[i]);
+        if (r == 0)
+#pragma unroll
+            for (int j = 0; j < E; ++j) s_acc[wave][i][cl * E + j] = acc[i][j];
+    }
+    __syncthreads();
+    for (int at = threadIdx.x; at < GT * D; at += 256) {
+        const int i = at / D, d = at - i * D;
+        if (g0 + i >= a.group) break;
+        const float m0 = s_ml[0][i].x, m1 = s_ml[1][i].x, m2 = s_ml[2][i].x, m3 = s_ml[3][i].x;
+        const float mx = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+        const float sf = mx == -INFINITY ? 0.0f : mx;
+        const float w0 = __builtin_amdgcn_exp2f(m0 - sf), w1 = __builtin_amdgcn_exp2f(m1 - sf);
+        const float w2 = __builtin_amdgcn_exp2f(m2 - sf), w3 = __builtin_amdgcn_exp2f(m3 - sf);
+        const float o = s_acc[0][i][d] * w0 + s_acc[1][i][d] * w1 + s_acc[2][i][d] * w2 + s_acc[3][i][d] * w3;
+        const size_t part = (static_cast<size_t>(s) * n_heads + head0 + i) * a.nsplit + z;
+        a.part_acc[part * D + d] = o;
+        if (d == 0)
+            a.part_ml[part] = make_float2(mx, s_ml[0][i].y * w0 + s_ml[1][i].y * w1 + s_ml[2][i].y * w2 + s_ml[3][i].y * w3);
+    }
+}
+
+// Grid (head, sequence): the splits of a row joined, out = sum_z acc_z f_z /
+// sum_z l_z f_z with f_z = exp2(m_z - max m), in the order of the splits
+// within each of the 256 / (D / 4) groups of lanes, then over the groups.
+template <int D>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttend a) {
+    constexpr int L4 = D / 4;
+    constexpr int G = 256 / L4;
+    __shared__ float4 s_acc[G][L4];
+    __shared__ float s_l[G];
+    __shared__ float s_m[4];
+    const int h = blockIdx.x;
+    const int s = blockIdx.y;
+    const uint4 e = a.seen[s];
+    if (e.x == kPagedNone) return;
+    const uint32_t nvis = e.x;
+    const int n = static_cast<int>((nvis + split_keys(nvis, a.nsplit) - 1) / split_keys(nvis, a.nsplit));
+    const size_t part = (static_cast<size_t>(s) * gridDim.x + h) * a.nsplit;
+    float m = -INFINITY;
+    for (int z = threadIdx.x; z < n; z += 256) m = fmaxf(m, a.part_ml[part + z].x);
+    m = wave_max_f_full(m);
+    if ((threadIdx.x & 63) == 0) s_m[threadIdx.x >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+    const float sf = m == -INFINITY ? 0.0f : m;
+    const int gi = threadIdx.x / L4;
+    const int d4 = threadIdx.x % L4;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float l = 0.0f;
+#pragma unroll 4
+    for (int z = gi; z < n; z += G) {
+        const float2 ml = a.part_ml[part + z];
+        const float4 v = reinterpret_cast<const float4*>(a.part_acc + (part + z) * D)[d4];
+        const float f = __builtin_amdgcn_exp2f(ml.x - sf);
+        l = fmaf(ml.y, f, l);
+        acc.x = fmaf(v.x, f, acc.x);
+        acc.y = fmaf(v.y, f, acc.y);
+        acc.z = fmaf(v.z, f, acc.z);
+        acc.w = fmaf(v.w, f, acc.w);
+    }
+    s_acc[gi][d4] = acc;
+    if (d4 == 0) s_l[gi] = l;
+    __syncthreads();
+    if (threadIdx.x < D) {
+        const float* f = reinterpret_cast<const float*>(s_acc);
+        float o = 0.0f, lt = 0.0f;
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+            o += f[i * D + threadIdx.x];
+            lt += s_l[i];
+        }
+        // no keys: zeros; keys whose scores are all -inf: 0 / 0, as the formula has it
+        a.out[static_cast<size_t>(s) * a.ldo + static_cast<size_t>(h) * D + threadIdx.x] = nvis == 0 ? 0.0f : o / lt;
+    }
+    if (a.lens_advance && h == 0 && threadIdx.x == 0 && e.w != 0) a.lens_advance[s] += 1;
+}
+
+// Grid (256 keys, key head, sequence): weights[key] += sum over the head's
+// query heads of exp2(score - M) / L, M and L joined from the splits again.
+__global__ __launch_bounds__(256) void paged_weights_kernel(PagedAttend a) {
+    __shared__ float2 s_ml[64];
+    const int hk = blockIdx.y;
+    const int s = blockIdx.z;
+    const uint4 e = a.seen[s];
+    if (e.x == kPagedNone) return;
+    const uint32_t nvis = e.x;
+    if (blockIdx.x * 256u >= nvis) return;
+    const int n = static_cast<int>((nvis + split_keys(nvis, a.nsplit) - 1) / split_keys(nvis, a.nsplit));
+    const size_t n_heads = static_cast<size_t>(gridDim.y) * a.group;
+    const size_t head0 = static_cast<size_t>(s) * n_heads + static_cast<size_t>(hk) * a.group;
+    for (int i = threadIdx.x >> 6; i < a.group; i += 4) {  // a wave a head
+        const float2* ml = a.part_ml + (head0 + i) * a.nsplit;
+        float m = -INFINITY, l = 0.0f;
+        for (int z = threadIdx.x & 63; z < n; z += 64) m = fmaxf(m, ml[z].x);
+        m = wave_max_f_full(m);
+        const float sf = m == -INFINITY ? 0.0f : m;
+        for (int z = threadIdx.x & 63; z < n; z += 64) l = fmaf(ml[z].y, __builtin_amdgcn_exp2f(ml[z].x - sf), l);
+        l = wave_sum_f_full(l);
+        if ((threadIdx.x & 63) == 0) s_ml[i] = make_float2(sf, l);
+    }
+    __syncthreads();
+    const uint32_t j = blockIdx.x * 256u + threadIdx.x;
+    if (j >= nvis) return;
+    float w = 0.0f;
+    for (int i = 0; i < a.group; ++i) {
+        const float sc = a.scores[(head0 + i) * a.score_ld + j];
+        w += __builtin_amdgcn_exp2f(sc - s_ml[i].x) / s_ml[i].y;
+    }
+    const uint32_t key = j < e.y ? j : j + e.z;
+    a.weights[(static_cast<size_t>(s) * gridDim.y + hk) * a.ldw + key] += w;
+}
+
+// Rows of k / v [rows][kv_heads * D] into the slots (seq, pos) of the cache;
+// a thread takes 16 bytes of a row.
+template <typename T>
+__global__ __launch_bounds__(256) void paged_write_kernel(PoolGeom g, int D, const float* __restrict__ k,
+                                                          const float* __restrict__ v, size_t ld, size_t rows,
+                                                          const uint32_t* seq, const uint32_t* pos,
+                                                          const uint32_t* tables, int n_seqs, size_t max_pages) {
+    constexpr int E = Row16<T>::N;
+    const int C = D / E;
+    const size_t per = static_cast<size_t>(g.kv_heads) * C;
+    const size_t at = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
+    const size_t row = at / per;
+    if (row >= rows) return;
+    const uint32_t hk = static_cast<uint32_t>((at - row * per) / C);
+    const int cl = static_cast<int>((at - row * per) % C);
+    const uint32_t p = pos[row];
+    const uint32_t s = seq ? seq[row] : static_cast<uint32_t>(row);
+    if (p == kPagedNone || s >= static_cast<uint32_t>(n_seqs) || (p >> g.page_shift) >= max_pages) return;
+    const PagedTables t{tables, nullptr, n_seqs, max_pages, 0};
+    const uint32_t dst = row_of(t, g, static_cast<int>(s), hk, p);
+    if (dst == kBadRow) return;
+    const size_t src = row * ld + static_cast<size_t>(hk) * D + static_cast<size_t>(cl) * E;
+    float f[E];
+#pragma unroll
+    for (int j = 0; j < E; ++j) f[j] = k[src + j];
+    static_cast<u4*>(g.k)[static_cast<size_t>(dst) * C + cl] = Row16<T>::pack(f);
+#pragma unroll
+    for (int j = 0; j < E; ++j) f[j] = v[src + j];
+    static_cast<u4*>(g.v)[static_cast<size_t>(dst) * C + cl] = Row16<T>::pack(f);
+}
+
+// ---- eviction --------------------------------------------------------------------
+
+// A weight as a whole number of the same order: NaN lowest, -0 as +0.
+__device__ __forceinline__ uint32_t weight_key(float v) {
+    if (v != v) return 0u;
+    if (v == 0.0f) v = 0.0f;
+    const uint32_t u = __float_as_uint(v);
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+// Grid (key head, sequence): the threshold by four passes over 8 bits of the
+// keys each (a histogram of the keys that share the bits found so far), then
+// the slots that stay in order: those above the threshold, and of those at it
+// the first ones.
+__global__ __launch_bounds__(1024) void paged_select_kernel(PagedEvict a, uint32_t kv_heads) {
+    __shared__ uint32_t s_hist[256];
+    __shared__ uint32_t s_pick[2];  // the digit, and how many are wanted within it
+    __shared__ uint32_t s_above[16], s_equal[16];
+    const int hk = blockIdx.x;
+    const int s = blockIdx.y;
+    const Cut c = cut_of(a, s);
+    if (hk == 0 && threadIdx.x == 0) a.dst_lens[s] = c.none ? kPagedNone : min(c.n, a.budget);
+    if (c.none) return;
+    const size_t row = static_cast<size_t>(s) * kv_heads + hk;
+    const float* w = a.weights + row * a.ldw;
+    uint32_t* kept = a.kept + row * a.budget;
+    float* dw = a.dst_weights + row * a.dst_ldw;
+    if (c.whole) {
+        for (uint32_t j = threadIdx.x; j < c.n; j += 1024) {
+            kept[j] = j;
+            dw[j] = w[j];
+        }
+        return;
+    }
+    uint32_t found = 0, want = c.want;  // the threshold's bits so far; how many of the keys that share them stay
+    for (int shift = 24; shift >= 0 && want; shift -= 8) {
+        if (threadIdx.x < 256) s_hist[threadIdx.x] = 0;
+        __syncthreads();
+        for (uint32_t j = c.lo + threadIdx.x; j < c.hi; j += 1024) {
+            const uint32_t k = weight_key(w[j]);
+            if (shift == 24 || (k >> (shift + 8)) == (found >> (shift + 8))) atomicAdd(&s_hist[(k >> shift) & 255u], 1u);
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            uint32_t left = want;
+            int b = 255;
+            for (; b > 0 && s_hist[b] < left; --b) left -= s_hist[b];
+            s_pick[0] = static_cast<uint32_t>(b);
+            s_pick[1] = left;
+        }
+        __syncthreads();
+        found |= s_pick[0] << shift;
+        want = s_pick[1];
+    }
+    // want: how many at the threshold stay (0: none is wanted at all)
+    const bool any = c.want != 0;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    uint32_t base = 0, equal_base = 0;
+    for (uint32_t j0 = 0; j0 < c.n; j0 += 1024) {
+        const uint32_t j = j0 + threadIdx.x;
+        const float v = j < c.n ? w[j] : 0.0f;
+        const bool middle = j >= c.lo && j < c.hi;
+        const uint32_t k = weight_key(v);
+        const bool above = j < c.n && (!middle || (any && k > found));
+        const bool equal = any && middle && k == found;
+        const uint64_t ma = __ballot(above), me = __ballot(equal);
+        if (lane == 0) {
+            s_above[wave] = __popcll(ma);
+            s_equal[wave] = __popcll(me);
+        }
+        __syncthreads();
+        uint32_t wa = 0, we = 0, ta = 0, te = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            if (i < wave) {
+                wa += s_above[i];
+                we += s_equal[i];
+            }
+            ta += s_above[i];
+            te += s_equal[i];
+        }
+        const uint64_t below = (1ull << lane) - 1;
+        const uint32_t e0 = equal_base + we + __popcll(me & below);  // equal ones before this slot
+        const bool stay = above || (equal && e0 < want);
+        if (stay) {
+            const uint32_t to = base + wa + __popcll(ma & below) + (min(e0, want) - min(equal_base, want));
+            kept[to] = j;
+            dw[to] = v;
+        }
+        base += ta + (min(equal_base + te, want) - min(equal_base, want));
+        equal_base += te;
+        __syncthreads();
+    }
+}
+
+// Grid (tile of kept slots, key head, sequence): their rows into the pages of
+// dst_tables, 16 bytes a lane.
+template <int C>
+__global__ __launch_bounds__(256) void paged_gather_kernel(PoolGeom g, PagedEvict a) {
+    constexpr int R = 256 / C;  // rows a step
+    constexpr int U = 4;
+    const int hk = blockIdx.y;
+    const int s = blockIdx.z;
+    const uint32_t len = a.t.lens[s];
+    if (len == kPagedNone) return;
+    const uint32_t n = min(min(len, a.t.max_len), a.budget);
+    const uint32_t i0 = blockIdx.x * (R * U);
+    if (i0 >= n) return;
+    const int cl = threadIdx.x % C;
+    const uint32_t* kept = a.kept + (static_cast<size_t>(s) * g.kv_heads + hk) * a.budget;
+    const PagedTables dst{a.dst_tables, nullptr, a.t.n_seqs, a.dst_max_pages, 0};
+    uint32_t from[U], to[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t i = i0 + u * R + threadIdx.x / C;
+        from[u] = to[u] = kBadRow;
+        if (i < n) {
+            from[u] = row_of(a.t, g, s, hk, kept[i]);
+            to[u] = row_of(dst, g, s, hk, i);
+        }
+        if (from[u] == kBadRow) to[u] = kBadRow;
+    }
+    u4 kw[U], vw[U];
+    const u4* kp = static_cast<const u4*>(g.k) + cl;
+    const u4* vp = static_cast<const u4*>(g.v) + cl;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (to[u] != kBadRow) {
+            kw[u] = kp[static_cast<size_t>(from[u]) * C];
+            vw[u] = vp[static_cast<size_t>(from[u]) * C];
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (to[u] != kBadRow) {
+            static_cast<u4*>(g.k)[static_cast<size_t>(to[u]) * C + cl] = kw[u];
+            static_cast<u4*>(g.v)[static_cast<size_t>(to[u]) * C + cl] = vw[u];
+        }
+    }
+}
+
+// ---- checks, for calls that ask for them ---------------------------------------------
+
+__device__ __forceinline__ void fault(unsigned long long* err, uint32_t row, int code) {
+    atomicMin(err, (static_cast<unsigned long long>(row) << 8) | static_cast<unsigned long long>(code));
+}
+
+__global__ void paged_check_kernel(PoolGeom g, PagedTables t, uint32_t add, const uint32_t* prefix, uint32_t window,
+                                   unsigned long long* err) {
+    const int s = blockIdx.x;
+    const uint32_t len = t.lens[s];
+    if (len == kPagedNone) return;
+    if (len > t.max_len || t.max_len - len < add) {
+        if (threadIdx.x == 0) fault(err, s, kFaultLen);
+        return;
+    }
+    const Seen e = seen_of(t, prefix, window, add != 0, s);
+    const uint32_t unit = 1u << g.page_shift;
+    // every page that holds a key that is seen
+    for (uint32_t pg = threadIdx.x; static_cast<uint64_t>(pg) * unit < e.n; pg += blockDim.x) {
+        const uint32_t first = pg * unit, last = min(first + unit, e.n);
+        const bool used = first < e.p || last > e.p + e.shift;
+        if (used && t.tables[static_cast<size_t>(s) * t.max_pages + pg] >= g.n_pages) fault(err, s, kFaultPage);
+    }
+}
+
+__global__ void paged_check_rows_kernel(PoolGeom g, size_t rows, const uint32_t* seq, const uint32_t* pos,
+                                        const uint32_t* tables, int n_seqs, size_t max_pages,
+                                        unsigned long long* err) {
+    const size_t row = static_cast<size_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+    if (row >= rows) return;
+    const uint32_t p = pos[row];
+    if (p == kPagedNone) return;
+    const uint32_t s = seq ? seq[row] : static_cast<uint32_t>(row);
+    const uint32_t at = static_cast<uint32_t>(row);
+    if (s >= static_cast<uint32_t>(n_seqs)) return fault(err, at, kFaultSeq);
+    if ((p >> g.page_shift) >= max_pages) return fault(err, at, kFaultLen);
+    if (tables[static_cast<size_t>(s) * max_pages + (p >> g.page_shift)] >= g.n_pages) fault(err, at, kFaultPage);
+}
+
+__global__ void clear_words_kernel(uint32_t* p, size_t n) {
+    const size_t i = static_cast<size_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+    if (i < n) p[i] = 0u;
+}
+
+// marks: a bit for every page that a sequence reads
+__global__ void paged_mark_kernel(PoolGeom g, PagedTables t, uint32_t* marks) {
+    const int s = blockIdx.x;
+    const uint32_t len = t.lens[s];
+    if (len == kPagedNone) return;
+    const uint32_t n = min(len, t.max_len);
+    for (uint32_t pg = threadIdx.x; (static_cast<uint64_t>(pg) << g.page_shift) < n; pg += blockDim.x) {
+        const uint32_t page = t.tables[static_cast<size_t>(s) * t.max_pages + pg];
+        if (page < g.n_pages) atomicOr(marks + (page >> 5), 1u << (page & 31));
+    }
+}
+
+// the pages written: of the pool, read by none, each written once
+__global__ void paged_check_dst_kernel(PoolGeom g, PagedEvict a, uint32_t* marks, unsigned long long* err) {
+    const int s = blockIdx.x;
+    const uint32_t len = a.t.lens[s];
+    if (len == kPagedNone) return;
+    const uint32_t n = min(min(len, a.t.max_len), a.budget);
+    for (uint32_t pg = threadIdx.x; (static_cast<uint64_t>(pg) << g.page_shift) < n; pg += blockDim.x) {
+        const uint32_t page = a.dst_tables[static_cast<size_t>(s) * a.dst_max_pages + pg];
+        if (page >= g.n_pages) {
+            fault(err, s, kFaultDstPage);
+            continue;
+        }
+        if (atomicOr(marks + (page >> 5), 1u << (page & 31)) & (1u << (page & 31))) fault(err, s, kFaultDstShared);
+    }
+}
+
+template <typename T, int D>
+void attend(hipStream_t s, const focr_hip_paged* c, const PagedAttend& a) {
+    const PoolGeom g = geom_of(c);
+    const int kv = static_cast<int>(c->n_kv_heads);
+    const auto grid = [&](int gt) { return dim3(a.nsplit, kv * ((a.group + gt - 1) / gt), a.t.n_seqs); };
+    if (a.group == 1)
+        FOCR_LAUNCH((paged_attend_kernel<T, D, 1, 8>), grid(1), dim3(256), 0, s, g, a);
+    else if (a.group == 2)
+        FOCR_LAUNCH((paged_attend_kernel<T, D, 2, 8>), grid(2), dim3(256), 0, s, g, a);
+    else if (a.group <= 4)
+        FOCR_LAUNCH((paged_attend_kernel<T, D, 4, 4>), grid(4), dim3(256), 0, s, g, a);
+    else
+        FOCR_LAUNCH((paged_attend_kernel<T, D, 8, 4>), grid(8), dim3(256), 0, s, g, a);
+}
+
+template <typename T>
+void attend_dim(hipStream_t s, const focr_hip_paged* c, const PagedAttend& a) {
+    if (c->head_dim == 64)
+        attend<T, 64>(s, c, a);
+    else if (c->head_dim == 128)
+        attend<T, 128>(s, c, a);
+    else
+        attend<T, 256>(s, c, a);
+}
+
+}  // namespace
+
+int paged_pick_splits(size_t n_seqs, size_t kv_heads, int group, uint32_t max_seen, int cu_count) {
+    return pick_splits(n_seqs, kv_heads, group, max_seen, cu_count);
+}
+
+hipError_t launch_paged_attend(hipStream_t s, const focr_hip_paged* c, const PagedAttend& a, focr_hip_ctx* ctx) {
+    const int kv = static_cast<int>(c->n_kv_heads);
+    {
+        ProfScope ps(ctx, "paged_attend");
+        if (c->dtype == FOCR_HIP_DT_F32)
+            attend_dim<float>(s, c, a);
+        else if (c->dtype == FOCR_HIP_DT_F16)
+            attend_dim<_Float16>(s, c, a);
+        else
+            attend_dim<__bf16>(s, c, a);
+    }
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    if (a.weights) {
+        ProfScope ps(ctx, "paged_weights");
+        FOCR_LAUNCH(paged_weights_kernel, dim3((a.t.max_len + 255) / 256, kv, a.t.n_seqs), dim3(256), 0, s, a);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
+    ProfScope ps(ctx, "paged_join");
+    const dim3 grid(kv * a.group, a.t.n_seqs);
+    if (c->head_dim == 64)
+        FOCR_LAUNCH(paged_join_kernel<64>, grid, dim3(256), 0, s, a);
+    else if (c->head_dim == 128)
+        FOCR_LAUNCH(paged_join_kernel<128>, grid, dim3(256), 0, s, a);
+    else
+        FOCR_LAUNCH(paged_join_kernel<256>, grid, dim3(256), 0, s, a);
+    return hipGetLastError();
+}
+
+hipError_t launch_paged_write(hipStream_t s, const focr_hip_paged* c, const float* k, const float* v, size_t ld,
+                              size_t rows, const uint32_t* seq, const uint32_t* pos, const uint32_t* tables,
+                              int n_seqs, size_t max_pages) {
+    const PoolGeom g = geom_of(c);
+    const int D = static_cast<int>(c->head_dim);
+    const size_t units = rows * c->n_kv_heads * c->head_dim * c->esize() / 16;
+    const dim3 grid(static_cast<uint32_t>((units + 255) / 256));
+    if (c->dtype == FOCR_HIP_DT_F32)
+        FOCR_LAUNCH(paged_write_kernel<float>, grid, dim3(256), 0, s, g, D, k, v, ld, rows, seq, pos, tables, n_seqs,
+                    max_pages);
+    else if (c->dtype == FOCR_HIP_DT_F16)
+        FOCR_LAUNCH(paged_write_kernel<_Float16>, grid, dim3(256), 0, s, g, D, k, v, ld, rows, seq, pos, tables,
+                    n_seqs, max_pages);
+    else
+        FOCR_LAUNCH(paged_write_kernel<__bf16>, grid, dim3(256), 0, s, g, D, k, v, ld, rows, seq, pos, tables, n_seqs,
+                    max_pages);
+    return hipGetLastError();
+}
+
+hipError_t launch_paged_evict(hipStream_t s, const focr_hip_paged* c, const PagedEvict& a, focr_hip_ctx* ctx) {
+    const PoolGeom g = geom_of(c);
+    {
+        ProfScope ps(ctx, "paged_select");
+        FOCR_LAUNCH(paged_select_kernel, dim3(g.kv_heads, a.t.n_seqs), dim3(1024), 0, s, a, g.kv_heads);
+    }
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    ProfScope ps(ctx, "paged_gather");
+    const uint32_t most = std::min(a.budget, a.t.max_len);
+    const int lanes = static_cast<int>(c->head_dim * c->esize() / 16);
+    const uint32_t rows = 4 * (256 / lanes);
+    const dim3 grid((most + rows - 1) / rows, g.kv_heads, a.t.n_seqs);
+    if (lanes == 8)
+        FOCR_LAUNCH(paged_gather_kernel<8>, grid, dim3(256), 0, s, g, a);
+    else if (lanes == 16)
+        FOCR_LAUNCH(paged_gather_kernel<16>, grid, dim3(256), 0, s, g, a);
+    else if (lanes == 32)
+        FOCR_LAUNCH(paged_gather_kernel<32>, grid, dim3(256), 0, s, g, a);
+    else
+        FOCR_LAUNCH(paged_gather_kernel<64>, grid, dim3(256), 0, s, g, a);
+    return hipGetLastError();
+}
+
+hipError_t launch_paged_check(hipStream_t s, const focr_hip_paged* c, const PagedTables& t, uint32_t add,
+                              const uint32_t* prefix, uint32_t window, unsigned long long* err) {
+    FOCR_LAUNCH(paged_check_kernel, dim3(t.n_seqs), dim3(256), 0, s, geom_of(c), t, add, prefix, window, err);
+    return hipGetLastError();
+}
+
+hipError_t launch_paged_check_rows(hipStream_t s, const focr_hip_paged* c, size_t rows, const uint32_t* seq,
+                                   const uint32_t* pos, const uint32_t* tables, int n_seqs, size_t max_pages,
+                                   unsigned long long* err) {
+    FOCR_LAUNCH(paged_check_rows_kernel, dim3(static_cast<uint32_t>((rows + 255) / 256)), dim3(256), 0, s, geom_of(c),
+                rows, seq, pos, tables, n_seqs, max_pages, err);
+    return hipGetLastError();
+}
+
+hipError_t launch_clear_words(hipStream_t s, uint32_t* p, size_t n) {
+    FOCR_LAUNCH(clear_words_kernel, dim3(static_cast<uint32_t>((n + 255) / 256)), dim3(256), 0, s, p, n);
+    return hipGetLastError();
+}
+
+hipError_t launch_paged_check_dst(hipStream_t s, const focr_hip_paged* c, const PagedEvict& a, uint32_t* marks,
+                                  unsigned long long* err) {
+    const PoolGeom g = geom_of(c);
+    hipError_t e = launch_clear_words(s, marks, (c->n_pages + 31) / 32);
+    if (e != hipSuccess) return e;
+    FOCR_LAUNCH(paged_mark_kernel, dim3(a.t.n_seqs), dim3(256), 0, s, g, a.t, marks);
+    FOCR_LAUNCH(paged_check_dst_kernel, dim3(a.t.n_seqs), dim3(256), 0, s, g, a, marks, err);
+    return hipGetLastError();
+}
+
+}  // namespace focr

@@ -1,0 +1,104 @@
+// k_paged_index.hpp — which keys a call on the paged cache sees, how they are
+// split, where their rows lie, and what an eviction keeps. Plain integer
+// arithmetic, compiled for the device by k_paged.hip and for the host by the
+// test that walks its bounds.
+#pragma once
+
+#include <algorithm>
+#include <cstddef>
+#include <cstdint>
+
+#include "focr_internal.hpp"
+
+#ifdef __HIP__
+#define FOCR_INDEX __device__ __forceinline__
+#else
+#define FOCR_INDEX inline
+#endif
+
+namespace focr {
+namespace {
+
+constexpr uint32_t kBadRow = 0xFFFFFFFFu;  // no key (past the end, or a page that is none)
+
+FOCR_INDEX uint32_t umin32(uint32_t a, uint32_t b) { return a < b ? a : b; }
+FOCR_INDEX uint32_t umax32(uint32_t a, uint32_t b) { return a > b ? a : b; }
+
+struct PoolGeom {
+    void* k;
+    void* v;
+    uint32_t n_pages;
+    int page_shift;
+    uint32_t kv_heads;
+};
+
+// What sequence s's token sees: keys [0, p) and [p + shift, n), nvis of them.
+// own: the key that a step writes (the last one seen), or none.
+struct Seen {
+    uint32_t n, p, shift, nvis;
+    bool none, own;
+};
+
+FOCR_INDEX Seen seen_of(const PagedTables& t, const uint32_t* prefix, uint32_t window, bool step, int s) {
+    Seen e{};
+    const uint32_t len = t.lens[s];
+    e.none = len == kPagedNone;
+    if (e.none) return e;
+    e.own = step && len < t.max_len;
+    e.n = umin32(len, t.max_len) + (e.own ? 1u : 0u);
+    e.p = e.n;
+    e.nvis = e.n;
+    if (window != 0u && window < e.n) {
+        e.p = prefix ? umin32(prefix[s], e.n) : 0u;
+        const uint32_t w0 = umax32(e.n - window, e.p);
+        e.shift = w0 - e.p;
+        e.nvis = e.p + (e.n - w0);
+    }
+    return e;
+}
+
+// Keys of one split: the visible ones over at most nsplit splits, in whole units.
+FOCR_INDEX uint32_t split_keys(uint32_t nvis, int nsplit) {
+    const uint32_t each = (nvis + nsplit - 1) / nsplit;
+    return umax32((each + kPagedChunkUnit - 1) / kPagedChunkUnit, 1u) * kPagedChunkUnit;
+}
+
+// Splits of a call. Enough blocks for every CU to hold several, splits of at
+// most kPagedChunkMax keys (their rows are kept in LDS) and of at least
+// kPagedChunkUnit.
+inline int pick_splits(size_t n_seqs, size_t kv_heads, int group, uint32_t max_seen, int cu_count) {
+    const size_t tiles = static_cast<size_t>((group + 7) / 8);
+    const size_t base = std::max<size_t>(n_seqs * kv_heads * tiles, 1);
+    const size_t least = (static_cast<size_t>(max_seen) + kPagedChunkMax - 1) / kPagedChunkMax;
+    const size_t most = (static_cast<size_t>(max_seen) + kPagedChunkUnit - 1) / kPagedChunkUnit;
+    const size_t fill = (8 * static_cast<size_t>(cu_count) + base - 1) / base;
+    return static_cast<int>(std::max<size_t>(std::min(std::max(fill, least), most), 1));
+}
+
+// The row (of head_dim elements) of key `key` of sequence s and head hk.
+FOCR_INDEX uint32_t row_of(const PagedTables& t, const PoolGeom& g, int s, uint32_t hk, uint32_t key) {
+    const uint32_t page = t.tables[static_cast<size_t>(s) * t.max_pages + (key >> g.page_shift)];
+    if (page >= g.n_pages) return kBadRow;
+    return ((page * g.kv_heads + hk) << g.page_shift) + (key & ((1u << g.page_shift) - 1u));
+}
+
+struct Cut {
+    uint32_t n, lo, hi, want;  // of the slots [lo, hi) the `want` heaviest stay, and all outside
+    bool none, whole;
+};
+
+FOCR_INDEX Cut cut_of(const PagedEvict& a, int s) {
+    Cut c{};
+    const uint32_t len = a.t.lens[s];
+    c.none = len == kPagedNone;
+    if (c.none) return c;
+    c.n = umin32(len, a.t.max_len);
+    c.whole = c.n <= a.budget;
+    c.lo = umin32(a.sinks, c.n);
+    c.hi = c.n - umin32(a.recent, c.n - c.lo);
+    c.want = c.whole ? c.hi - c.lo : a.budget - c.lo - (c.n - c.hi);
+    return c;
+}
+
+}  // namespace
+}  // namespace focr

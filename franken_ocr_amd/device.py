@@ -146,6 +146,15 @@ class DeviceArray:
         a._p = ptr
         return a
 
+    @classmethod
+    def borrow(cls, ctx: Context, ptr: int, shape, dtype, owner=None) -> "DeviceArray":
+        """Device memory that something else owns, as a DeviceArray (it frees
+        nothing; `owner`, if given, is kept alive). Work of other streams on
+        it is the caller's to order."""
+        a = cls.adopt(ctx, C.c_void_p(int(ptr)), shape, dtype)
+        a._borrowed = owner if owner is not None else True
+        return a
+
     @property
     def ptr(self) -> int:
         return int(self._p.value or 0)

@@ -9,7 +9,10 @@ Mirrors, on uploaded weights and device arrays:
   sampler.rs:168-186),
 * ``MoeLayer.route`` / ``MoeLayer.decode`` (moe.rs:181-266,
   decoder.rs:2199-2268),
-* ``RingCache`` (rswa.rs:121-152, :389-513, :894-939, :1320-1367).
+* ``RingCache`` (rswa.rs:121-152, :389-513, :894-939, :1320-1367),
+
+and, without a counterpart in the reference, ``PagedCache`` (attention over and
+eviction from a paged cache) and ``beam_select`` / ``beam_reorder``.
 
 All work is queued on the context's stream; results come back with
 ``DeviceArray.numpy()``.
@@ -368,6 +371,193 @@ class RingCache:
             self.free()
         except Exception:
             pass
+
+
+_PAGED_DTYPES = {"f32": _abi.DT_F32, "f16": _abi.DT_F16, "bf16": _abi.DT_BF16}
+NO_SEQUENCE = 0xFFFFFFFF  # a length (or write position) that means: nothing in this row
+
+
+class PagedCache:
+    """One layer's keys and values in pages, [n_pages, n_kv_heads, page_size,
+    head_dim] each, for sequences that may share pages.
+
+    The page tables [n_seqs, max_pages] u32 and lengths [n_seqs] u32 are device
+    arrays given with every call. ``dtype`` is "f32", "f16" or "bf16"; ``k`` and
+    ``v`` (DeviceArrays) make the cache use pools that exist already. Query,
+    key, value and output rows are f32; their row strides are the arrays' widths
+    unless given (``ldq``, ``ldkv``, ``ldo``, in floats)."""
+
+    def __init__(self, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int = HEAD_DIM, dtype: str = "f32",
+                 k: DeviceArray | None = None, v: DeviceArray | None = None, ctx: Context | None = None):
+        self.ctx = ctx or default_context()
+        self.n_pages, self.page_size = int(n_pages), int(page_size)
+        self.n_kv_heads, self.head_dim, self.dtype = int(n_kv_heads), int(head_dim), dtype
+        self._h = C.c_void_p()
+        if dtype not in _PAGED_DTYPES:
+            raise ValueError(f"PagedCache: dtype {dtype!r} is not one of {sorted(_PAGED_DTYPES)}")
+        need = self.n_pages * self.page_size * self.n_kv_heads * self.head_dim * (4 if dtype == "f32" else 2)
+        for pool in (k, v):
+            if pool is not None and pool.nbytes < need:
+                raise _abi.ContractViolation(_abi.E_SHAPE, f"PagedCache: a pool of {pool.nbytes} B for {need} B")
+        self._keep = (k, v)
+        _abi.call("focr_hip_paged_create", self.ctx.handle, self.n_pages, self.page_size, self.n_kv_heads,
+                  self.head_dim, _PAGED_DTYPES[dtype], _p(k), _p(v), C.byref(self._h))
+
+    def regions(self) -> dict:
+        """Device addresses of the pools."""
+        ptrs = [C.c_void_p(), C.c_void_p()]
+        _abi.call("focr_hip_paged_regions", self._h, *[C.byref(p) for p in ptrs])
+        return {"k": int(ptrs[0].value), "v": int(ptrs[1].value)}
+
+    def _rows(self, who: str, tables: DeviceArray, lens: DeviceArray):
+        n, wide = tables.shape
+        if lens.shape[0] != n:
+            raise _abi.ContractViolation(_abi.E_SHAPE, f"{who}: {lens.shape[0]} lengths for {n} rows of tables")
+        return n, wide
+
+    def _heads(self, who: str, q: DeviceArray, out: DeviceArray, n: int, n_heads, ldq, ldo):
+        heads = n_heads if n_heads is not None else q.shape[-1] // self.head_dim
+        for name, a, ld in (("q", q, ldq), ("out", out, ldo)):
+            self._fits(who, name, a, n, heads * self.head_dim, ld)
+        return heads, ldq or heads * self.head_dim, ldo or heads * self.head_dim
+
+    @staticmethod
+    def _fits(who: str, name: str, a, rows: int, wide: int, ld) -> None:
+        """The array holds `rows` rows of `wide` values, `ld` apart (a raw pointer is taken on trust)."""
+        if isinstance(a, DeviceArray) and rows and a.nbytes // a.dtype.itemsize < (rows - 1) * (ld or wide) + wide:
+            raise _abi.ContractViolation(_abi.E_SHAPE, f"{who}: {name} of shape {a.shape} holds no {rows} rows of {wide}")
+
+    def write(self, k: DeviceArray, v: DeviceArray, pos: DeviceArray, tables: DeviceArray,
+              seq: DeviceArray | None = None, ldkv: int | None = None, check: bool = False) -> None:
+        """Rows k / v [rows, n_kv_heads * head_dim] into slots pos[i] of the
+        sequences seq[i] (sequence i without seq); NO_SEQUENCE skips a row."""
+        n, wide = tables.shape
+        rows, row = pos.shape[0], self.n_kv_heads * self.head_dim
+        self._fits("paged_write", "k", k, rows, row, ldkv)
+        self._fits("paged_write", "v", v, rows, row, ldkv)
+        self._fits("paged_write", "seq", seq, rows, 1, None)
+        _abi.call("focr_hip_paged_write", self.ctx.handle, self._h, _p(k), _p(v), ldkv or row, rows, _p(seq), _p(pos),
+                  _p(tables), n, wide, 1 if check else 0)
+
+    def attention(self, q: DeviceArray, tables: DeviceArray, lens: DeviceArray, out: DeviceArray,
+                  max_len: int | None = None, prefix: DeviceArray | None = None, window: int = 0, scale: float = 0.0,
+                  weights: DeviceArray | None = None, n_heads: int | None = None, ldq: int | None = None,
+                  ldo: int | None = None, check: bool = False) -> None:
+        """q [n_seqs, n_heads * head_dim] over each sequence's lens[s] keys (at
+        most max_len, by default what the tables hold): all of them, or the
+        first prefix[s] and the last `window`. weights [n_seqs, n_kv_heads,
+        >= max_len] gathers the probabilities."""
+        n, wide = self._rows("paged_attention", tables, lens)
+        heads, ldq, ldo = self._heads("paged_attention", q, out, n, n_heads, ldq, ldo)
+        self._fits("paged_attention", "prefix", prefix, n, 1, None)
+        ldw = self._weights("paged_attention", weights, n)
+        _abi.call("focr_hip_paged_attention", self.ctx.handle, self._h, _p(q), ldq, heads, _p(tables), n, wide, _p(lens),
+                  wide * self.page_size if max_len is None else int(max_len), _p(prefix), int(window), float(scale),
+                  _p(out), ldo, _p(weights), ldw, 1 if check else 0)
+
+    def step(self, q: DeviceArray, k_steps: DeviceArray, v_steps: DeviceArray, tables: DeviceArray, lens: DeviceArray,
+             out: DeviceArray, max_len: int | None = None, prefix: DeviceArray | None = None, window: int = 0,
+             scale: float = 0.0, weights: DeviceArray | None = None, n_heads: int | None = None, ldq: int | None = None,
+             ldkv: int | None = None, ldo: int | None = None, advance: bool = False, check: bool = False) -> None:
+        """Each sequence's new row written at slot lens[s], then the attention
+        over lens[s] + 1 keys; with advance the lengths are counted up."""
+        n, wide = self._rows("paged_step", tables, lens)
+        heads, ldq, ldo = self._heads("paged_step", q, out, n, n_heads, ldq, ldo)
+        row = self.n_kv_heads * self.head_dim
+        self._fits("paged_step", "k_steps", k_steps, n, row, ldkv)
+        self._fits("paged_step", "v_steps", v_steps, n, row, ldkv)
+        self._fits("paged_step", "prefix", prefix, n, 1, None)
+        ldw = self._weights("paged_step", weights, n)
+        _abi.call("focr_hip_paged_step", self.ctx.handle, self._h, _p(q), ldq, heads, _p(k_steps), _p(v_steps),
+                  ldkv or row, _p(tables), n, wide, _p(lens), wide * self.page_size if max_len is None else int(max_len),
+                  _p(prefix), int(window), float(scale), _p(out), ldo, _p(weights), ldw, 1 if advance else 0,
+                  1 if check else 0)
+
+    def _weights(self, who: str, weights, n: int) -> int:
+        if weights is None:
+            return 0
+        if len(weights.shape) != 3 or weights.shape[0] < n or weights.shape[1] != self.n_kv_heads:
+            raise _abi.ContractViolation(_abi.E_SHAPE, f"{who}: weights of shape {weights.shape} are not "
+                                                       f"[{n}, {self.n_kv_heads}, slots]")
+        return weights.shape[2]
+
+    def evict(self, tables: DeviceArray, lens: DeviceArray, weights: DeviceArray, budget: int, dst_tables: DeviceArray,
+              dst_lens: DeviceArray, dst_weights: DeviceArray, sinks: int = 0, recent: int = 0,
+              max_len: int | None = None, kept: DeviceArray | None = None, check: bool = False) -> None:
+        """Each sequence cut to `budget` slots per key head — the first `sinks`,
+        the last `recent` and the heaviest of the rest — in order, in the pages
+        of dst_tables. kept [n_seqs, n_kv_heads, budget] receives the slots."""
+        n, wide = self._rows("paged_evict", tables, lens)
+        most = wide * self.page_size if max_len is None else int(max_len)
+        ldw = self._weights("paged_evict", weights, n)
+        dst_ldw = self._weights("paged_evict", dst_weights, n)
+        self._fits("paged_evict", "dst_lens", dst_lens, n, 1, None)
+        self._fits("paged_evict", "kept", kept, n * self.n_kv_heads, int(budget), None)
+        if dst_tables.shape[0] < n:
+            raise _abi.ContractViolation(_abi.E_SHAPE, f"paged_evict: dst_tables of shape {dst_tables.shape} for {n} rows")
+        _abi.call("focr_hip_paged_evict", self.ctx.handle, self._h, _p(tables), n, wide, _p(lens),
+                  min(most, ldw) if max_len is None else most, _p(weights), ldw, int(budget), int(sinks), int(recent),
+                  _p(dst_tables), dst_tables.shape[1], _p(dst_lens), _p(dst_weights), dst_ldw, _p(kept),
+                  1 if check else 0)
+
+    def free(self) -> None:
+        if self._h:
+            _abi.lib().focr_hip_paged_free(self._h)
+            self._h = C.c_void_p()
+
+    def __del__(self):  # pragma: no cover
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+def beam_select(logits: DeviceArray, scores: DeviceArray, beams: int, parents: DeviceArray, tokens: DeviceArray,
+                new_scores: DeviceArray, done: DeviceArray | None = None, new_done: DeviceArray | None = None,
+                history: DeviceArray | None = None, history_len: DeviceArray | None = None, ngram_size: int = 0,
+                window: int = NGRAM_WINDOW_SINGLE, whitelist: DeviceArray | None = None,
+                eos: int = DEFAULT_EOS_TOKEN_ID, check: bool = False) -> None:
+    """One step of beam search over logits [groups * beams, vocab] and scores
+    [groups * beams]: parents (the beam within its group), tokens, new_scores
+    and new_done of the chosen continuations. ngram_size > 0 applies the
+    no-repeat-ngram ban of the sampler to each beam's history."""
+    rows, vocab = logits.shape
+    beams = int(beams)
+    if beams <= 0 or rows % beams:
+        raise _abi.ContractViolation(_abi.E_SHAPE, f"beam_select: {rows} rows are no groups of {beams}")
+    for name, a in (("scores", scores), ("parents", parents), ("tokens", tokens), ("new_scores", new_scores),
+                    ("done", done), ("new_done", new_done), ("history_len", history_len)):
+        PagedCache._fits("beam_select", name, a, rows, 1, None)
+    cap = history.shape[1] if history is not None else 0
+    PagedCache._fits("beam_select", "history", history, rows, cap, None)
+    nw = whitelist.shape[0] if whitelist is not None else 0
+    _abi.call("focr_hip_beam_select", logits.ctx.handle, _p(logits), vocab, rows // beams, beams, vocab, _p(scores),
+              _p(done), int(eos), _p(history), cap, _p(history_len), int(ngram_size), int(window), _p(whitelist), nw,
+              _p(parents), _p(tokens), _p(new_scores), _p(new_done), 1 if check else 0)
+
+
+def beam_reorder(parents: DeviceArray, beams: int, tokens: DeviceArray | None = None,
+                 history: DeviceArray | None = None, history_len: DeviceArray | None = None, advance: bool = False,
+                 caches: list[PagedCache] = (), tables: DeviceArray | None = None, lens: DeviceArray | None = None,
+                 rings: list[RingCache] = (), check: bool = False) -> None:
+    """The states of the chosen beams put where their slots are, in place: slot
+    b of each group takes slot parents[b]'s history (then tokens[b] behind it),
+    the entries of its page table up to the page in progress and that page's
+    rows in every cache (one per layer, sharing the tables), and its rings."""
+    rows, beams = parents.shape[0], int(beams)
+    if beams <= 0 or rows % beams:
+        raise _abi.ContractViolation(_abi.E_SHAPE, f"beam_reorder: {rows} rows are no groups of {beams}")
+    for name, a in (("tokens", tokens), ("history_len", history_len), ("lens", lens)):
+        PagedCache._fits("beam_reorder", name, a, rows, 1, None)
+    cap = history.shape[1] if history is not None else 0
+    wide = tables.shape[1] if tables is not None else 0
+    PagedCache._fits("beam_reorder", "history", history, rows, cap, None)
+    PagedCache._fits("beam_reorder", "tables", tables, rows, wide, None)
+    paged = (C.c_void_p * len(caches))(*[c._h.value for c in caches])
+    ring = (C.c_void_p * len(rings))(*[c._h.value for c in rings])
+    _abi.call("focr_hip_beam_reorder", parents.ctx.handle, rows // beams, beams, _p(parents), _p(tokens), _p(history),
+              cap, _p(history_len), 1 if advance else 0, C.cast(paged, C.c_void_p), len(caches), _p(tables), wide,
+              _p(lens), C.cast(ring, C.c_void_p), len(rings), 1 if check else 0)
 
 
 def prefill_chunk_bounds(seq: int, chunk: int) -> list:

@@ -64,6 +64,7 @@ typedef struct focr_hip_moe_layer_i4 focr_hip_moe_layer_i4;
 typedef struct focr_hip_decoder_layer focr_hip_decoder_layer;
 typedef struct focr_hip_decoder focr_hip_decoder;
 typedef struct focr_hip_rswa focr_hip_rswa;
+typedef struct focr_hip_paged focr_hip_paged;
 typedef struct focr_hip_focrq focr_hip_focrq;
 typedef struct focr_hip_focrq_writer focr_hip_focrq_writer;
 
@@ -425,6 +426,127 @@ int32_t focr_hip_rswa_set_state(focr_hip_rswa* cache, size_t stream, uint32_t ri
 /* Device pointers of one stream's regions (for direct fills/readback). */
 int32_t focr_hip_rswa_regions(const focr_hip_rswa* cache, size_t stream, float** ref_k,
                               float** ref_v, float** ring_k, float** ring_v);
+
+/* ---- paged key-value cache -------------------------------------------------
+ * No counterpart in the reference (its caches are the R-SWA rings above): one
+ * layer's keys and values in pages, for sequences of any length that may share
+ * pages (beams of one prompt), with grouped heads, in f32, f16 or bf16.
+ * K and V pools [n_pages][n_kv_heads][page_size][head_dim]; slot j of sequence
+ * s is slot j % page_size of page tables[s][j / page_size]. The tables
+ * [n_seqs][max_pages] and the lengths [n_seqs] are the caller's device arrays,
+ * so a captured step replays while they grow; a length of 0xFFFFFFFF means that
+ * the row holds no sequence: nothing of it is read or written, its output row
+ * stays as it is. Scratch comes from the context: the first call of a size
+ * allocates it (make it before a capture; a capture that would allocate gets
+ * E_STATE). Graphs captured from one context share its scratch, so they must
+ * not run at the same time; use a context for each that does.
+ * check = 1 waits for the stream, looks at what the tables and lengths hold
+ * and returns E_STATE (a length past max_len or the tables) or E_SHAPE (a page
+ * that is none) before anything is written. With check = 0 a length is cut to
+ * max_len and a slot on a page that is none is not read or written. */
+/* Pools of the handle's own (zeroed; k_pool and v_pool null) or of the
+ * caller's (16-byte aligned device arrays, not freed). dtype FOCR_HIP_DT_F32,
+ * _F16 or _BF16; page_size a power of two up to 1024; head_dim 64, 128 or 256;
+ * n_pages * n_kv_heads * page_size < 2^32 - 1. */
+int32_t focr_hip_paged_create(focr_hip_ctx* ctx, size_t n_pages, size_t page_size, size_t n_kv_heads,
+                              size_t head_dim, int32_t dtype, void* k_pool, void* v_pool,
+                              focr_hip_paged** out);
+int32_t focr_hip_paged_free(focr_hip_paged* cache);
+/* Device pointers of the pools (for direct fills and readback). */
+int32_t focr_hip_paged_regions(const focr_hip_paged* cache, void** k_pool, void** v_pool);
+/* Rows k / v [rows][n_kv_heads * head_dim] f32, ld floats apart (a prompt's or
+ * a step's), rounded to the cache's type (to nearest, ties to even) into slot
+ * pos[i] of sequence seq[i] (seq null: sequence i). A pos of 0xFFFFFFFF skips
+ * the row. Two rows of one call must not go to the same slot. */
+int32_t focr_hip_paged_write(focr_hip_ctx* ctx, focr_hip_paged* cache, const float* k, const float* v,
+                             size_t ld, size_t rows, const uint32_t* seq, const uint32_t* pos,
+                             const uint32_t* tables, size_t n_seqs, size_t max_pages, int32_t check);
+/* One query row per sequence over its cache: q [n_seqs][n_heads * head_dim]
+ * f32 (rows ldq floats apart), n_heads 1 .. 64 times n_kv_heads, query head h
+ * reads key head h / (n_heads / n_kv_heads). Of the n = lens[s] keys (at most
+ * max_len, which is what the call is sized for) it sees all (window 0), or the
+ * first min(prefix[s], n) (prefix null: none) and the last `window` — with the
+ * prompt's length as prefix and a window of 128 what the R-SWA ring sees. out
+ * [n_seqs][n_heads * head_dim] (rows ldo apart) = softmax(scale q.k) v, scale
+ * 0 meaning 1 / sqrt(head_dim); zeros where there is no key. The sums are f32,
+ * and the same call gives the same bits. weights (nullable)
+ * [n_seqs][n_kv_heads][ldw], ldw >= max_len: every key that is seen has the
+ * probabilities of its key head's query heads added. */
+int32_t focr_hip_paged_attention(focr_hip_ctx* ctx, const focr_hip_paged* cache, const float* q, size_t ldq,
+                                 size_t n_heads, const uint32_t* tables, size_t n_seqs, size_t max_pages,
+                                 const uint32_t* lens, size_t max_len, const uint32_t* prefix,
+                                 size_t window, float scale, float* out, size_t ldo, float* weights,
+                                 size_t ldw, int32_t check);
+/* A decode step: each sequence's new row k_steps / v_steps [n_seqs][n_kv_heads
+ * * head_dim] (rows ldkv apart) written at slot lens[s] as by
+ * focr_hip_paged_write, then the attention over lens[s] + 1 keys, in the same
+ * launches. With advance = 1 the lengths are counted up on the device. A
+ * sequence that has max_len keys already gets no new one (E_STATE with
+ * check = 1). */
+int32_t focr_hip_paged_step(focr_hip_ctx* ctx, focr_hip_paged* cache, const float* q, size_t ldq,
+                            size_t n_heads, const float* k_steps, const float* v_steps, size_t ldkv,
+                            const uint32_t* tables, size_t n_seqs, size_t max_pages, uint32_t* lens,
+                            size_t max_len, const uint32_t* prefix, size_t window, float scale, float* out,
+                            size_t ldo, float* weights, size_t ldw, int32_t advance, int32_t check);
+/* Cuts caches to a budget by the weights that attention gathered. Of a
+ * sequence of n > budget slots, and for each key head by itself, there stay
+ * the first `sinks`, the last `recent`, and of the others the budget - sinks -
+ * recent of the most weight (equal ones: the lower slot; NaN below all); of n
+ * <= budget slots all. They keep their order: the i-th goes to slot i of the
+ * pages of dst_tables [n_seqs][dst_max_pages], which no sequence of the call
+ * may read and no two share (source pages may be shared, so nothing moves
+ * within them). dst_lens [n_seqs] = min(n, budget); dst_weights
+ * [n_seqs][n_kv_heads][dst_ldw] the weights of the slots that stay; kept
+ * (nullable) [n_seqs][n_kv_heads][budget] their slots. dst_lens may be lens.
+ * With several layers each has weights, so evicts, of its own; the lengths
+ * agree. */
+int32_t focr_hip_paged_evict(focr_hip_ctx* ctx, focr_hip_paged* cache, const uint32_t* tables, size_t n_seqs,
+                             size_t max_pages, const uint32_t* lens, size_t max_len, const float* weights,
+                             size_t ldw, size_t budget, size_t sinks, size_t recent,
+                             const uint32_t* dst_tables, size_t dst_max_pages, uint32_t* dst_lens,
+                             float* dst_weights, size_t dst_ldw, uint32_t* kept, int32_t check);
+
+/* ---- beam search -----------------------------------------------------------
+ * No counterpart in the reference (its sampler is greedy). Row g * beams + b
+ * is beam b of group g; beams <= 32. */
+/* One step's selection over logits [groups * beams][vocab] (rows ld apart) and
+ * scores [groups * beams] (log probabilities; -inf for a beam that is not
+ * there, as all but one of a group at its start): the candidates are score +
+ * (logit - log sum exp(the row's logits)), in f64, a NaN among the results
+ * counting as -inf; NaN logits are skipped, banned tokens (the ban of
+ * focr_hip_lm_head_sample_i8 on history / history_len, ngram_size 0: none) are
+ * no candidates but part of the sum. A beam with done[row] != 0 (nullable) has
+ * one candidate, eos_token_id at its score. The first `beams` of the order
+ * (score descending, beam ascending, logit descending, token ascending) give
+ * parents (the beam within its group), tokens, new_scores (may be scores) and
+ * new_done (nullable, may be done: the parent's, or token == eos_token_id).
+ * Slots left over take themselves, eos_token_id, -inf and done. check = 1
+ * reports a history_len over history_cap (E_SHAPE). */
+int32_t focr_hip_beam_select(focr_hip_ctx* ctx, const float* logits, size_t ld, size_t groups, size_t beams,
+                             size_t vocab, const float* scores, const uint8_t* done, uint32_t eos_token_id,
+                             const uint32_t* history, size_t history_cap, const uint32_t* history_len,
+                             size_t ngram_size, size_t window, const uint32_t* whitelist, size_t n_whitelist,
+                             uint32_t* parents, uint32_t* tokens, float* new_scores, uint8_t* new_done,
+                             int32_t check);
+/* The states of the chosen beams put where their slots are, in place: slot b
+ * of a group takes from slot parents[b]
+ *  - its history (nullable; [rows][history_cap]) and history_len; then
+ *    tokens[row] (nullable) is written behind it and, with advance = 1, counted;
+ *  - its entries of tables [rows][max_pages] (shared by the caches, one per
+ *    layer, of one page size) up to the page in progress of lens[row], the
+ *    same length throughout a group; the entry of that page and those after it
+ *    stay the slot's own, and the page takes the parent's rows;
+ *  - its ring's rows in each of `rings` (streams g * beams + b, with the same
+ *    prompt and the same cursors throughout a group, E_STATE otherwise).
+ * So the beams of a group may share the pages they have filled and must not
+ * share the one in progress. A parent that is not below beams is taken as the
+ * slot itself, a group whose lengths differ keeps its tables and pages;
+ * check = 1 reports these (E_SHAPE, E_STATE) before anything is written. */
+int32_t focr_hip_beam_reorder(focr_hip_ctx* ctx, size_t groups, size_t beams, const uint32_t* parents,
+                              const uint32_t* tokens, uint32_t* history, size_t history_cap,
+                              uint32_t* history_len, int32_t advance, focr_hip_paged* const* caches,
+                              size_t n_caches, uint32_t* tables, size_t max_pages, const uint32_t* lens,
+                              focr_hip_rswa* const* rings, size_t n_rings, int32_t check);
 
 /* nn.rs:240-253 rms_norm over rows x [rows, n] f32 -> y (device pointers; w
  * [n] device, nullable): y = (x * rstd) * w, rstd = 1 / sqrt(mean(x^2) + eps)

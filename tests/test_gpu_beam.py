@@ -1,0 +1,455 @@
+"""Beam search on the device: the selection against the definition in 64 bits,
+the reordered states exactly, and a search over paged and ring caches against
+the same search with every beam's states kept apart on the host.
+
+The order of candidates is tested exactly: scores that differ by less than
+1e-9 do not come up in the seeded draws (asserted), and equal ones are made
+equal by construction. new_scores is the f64 score rounded to f32: within
+2^-24 of it, and 1e-9 for the sum's and the exponentials' own roundings."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from franken_ocr_amd import _abi
+from test_gpu_paged import Host, _capture
+
+pytestmark = pytest.mark.gpu
+
+EOS = 1
+NONE = 0xFFFFFFFF
+
+
+def _say(msg):
+    print(f"[gpu-beam] {msg}", flush=True)
+
+
+def _bans(history, n, window):
+    """Tokens that would end an n-gram of the last `window` tokens again."""
+    size = len(history)
+    if n == 0 or size < n:
+        return set()
+    last, start = list(history[size - (n - 1):]) if n > 1 else [], max(0, size - window) if window else 0
+    return {history[i + n - 1] for i in range(start, size - n + 1) if list(history[i: i + n - 1]) == last}
+
+
+def _select(logits, scores, beams, done, banned):
+    """(parents, tokens, scores in f64) by the definition."""
+    rows, vocab = logits.shape
+    parents, tokens, new = [], [], []
+    for g in range(rows // beams):
+        found = []
+        for b in range(beams):
+            r = g * beams + b
+            s = float(scores[r])
+            if done[r]:
+                found.append((s if s == s else -np.inf, b, 0.0, EOS))
+                continue
+            x = logits[r].astype(np.float64)
+            ok = ~np.isnan(x)
+            with np.errstate(all="ignore"):
+                m = x[ok].max() if ok.any() else -np.inf
+                if np.isinf(m):
+                    total = m
+                else:
+                    total = m + np.log(np.exp(x[ok] - m).sum())
+                keep = ok.copy()
+                keep[[t for t in banned[r] if t < vocab]] = False
+                at = np.nonzero(keep)[0]
+                at = at[np.argsort(-x[at], kind="stable")[:beams]]
+                for t in at.tolist():
+                    c = s + (x[t] - total)
+                    found.append((c if c == c else -np.inf, b, x[t], t))
+        found.sort(key=lambda f: (-f[0], f[1], -f[2], f[3]))
+        near = [f[0] for f in found if np.isfinite(f[0])]
+        assert all(a == b or a - b > 1e-9 for a, b in zip(near, near[1:]))
+        for i in range(beams):
+            c, b, _, t = found[i] if i < len(found) else (-np.inf, i, 0.0, EOS)
+            parents.append(b)
+            tokens.append(t)
+            new.append(c)
+    return parents, tokens, np.array(new)
+
+
+def _run(ctx, logits, scores, beams, done=None, history=None, lens=None, check=True, **kw):
+    from franken_ocr_amd.engine import beam_select
+
+    rows = len(scores)
+    p, t = (ctx.to_device(np.full(rows, 77, np.uint32)) for _ in "pt")
+    ns, nd = ctx.empty((rows,), np.float32), ctx.empty((rows,), np.uint8)
+    dh = ctx.to_device(history) if history is not None else None
+    dl = ctx.to_device(np.array(lens, np.uint32)) if lens is not None else None
+    beam_select(ctx.to_device(logits), ctx.to_device(np.asarray(scores, np.float32)), beams, p, t, ns,
+                done=ctx.to_device(done) if done is not None else None, new_done=nd, history=dh, history_len=dl, eos=EOS,
+                check=check, **kw)
+    return p.numpy().tolist(), t.numpy().tolist(), ns.numpy(), nd.numpy().tolist()
+
+
+def _same(got, want, done, beams):
+    p, t, s, d = got
+    wp, wt, ws = want
+    assert p == wp and t == wt
+    fine = np.isfinite(ws)
+    assert np.array_equal(s[~fine], ws[~fine].astype(np.float32))
+    assert np.all(np.abs(s[fine] - ws[fine]) <= np.abs(ws[fine]) * 2.0 ** -24 + 1e-9)
+    assert d == [int(bool(done[i // beams * beams + q]) or x == EOS) for i, (q, x) in enumerate(zip(wp, wt))]
+
+
+@pytest.mark.parametrize("groups,beams,vocab", [(1, 1, 1), (1, 4, 129280), (3, 2, 4096), (2, 5, 4097), (2, 8, 50021),
+                                                (1, 32, 12289), (4, 3, 2), (2, 16, 7), (65, 1, 300), (1, 32, 8192)])
+def test_selection_against_64_bits(ctx, groups, beams, vocab):
+    _say(f"select {groups} x {beams} over {vocab}")
+    rng = np.random.default_rng(groups * 1000 + beams + vocab)
+    rows = groups * beams
+    logits = (3 * rng.standard_normal((rows, vocab))).astype(np.float32)
+    scores = (-3 * rng.random(rows)).astype(np.float32)
+    done = (rng.random(rows) < 0.2).astype(np.uint8)
+    got = _run(ctx, logits, scores, beams, done)
+    _same(got, _select(logits, scores, beams, done, [set()] * rows), done, beams)
+    assert _run(ctx, logits, scores, beams, done)[2].tobytes() == got[2].tobytes()
+
+
+def test_selection_of_odd_rows(ctx):
+    """Ties, NaN, infinities, rows with nothing, beams that are not there."""
+    _say("odd rows")
+    rng = np.random.default_rng(5)
+    beams, vocab = 4, 9000
+    x = (2 * rng.standard_normal((40, vocab))).astype(np.float32)
+    scores = (-2 * rng.random(40)).astype(np.float32)
+    done = np.zeros(40, np.uint8)
+    x[0:4] = x[0]                                       # group 0: the start, four times one row
+    scores[0:4] = [0.0, -np.inf, -np.inf, -np.inf]
+    x[4:8], scores[4:8] = x[4], scores[4]               # group 1: equal candidates in every beam
+    x[8, ::3] = np.nan                                  # group 2: NaN among the logits
+    x[9] = np.nan                                       # and nothing else
+    x[10] = -np.inf                                     # no probability anywhere
+    x[11, 100] = np.inf                                 # too much at one token
+    x[12:16] = 0.0                                      # group 3: every logit equal
+    x[12:16, 5::2] = -0.0
+    done[16:20] = 1                                     # group 4: all finished, equal scores among them
+    scores[17] = scores[18]
+    scores[20:24] = -np.inf                             # group 5: no beam is there
+    x[24:28] = np.nan                                   # group 6: nothing at all
+    done[24] = 1
+    x[28:32] = np.where(np.arange(vocab) < 3, x[28:32], np.nan)  # group 7: three tokens
+    x[29:32] = np.nan
+    x[32:36, 4095:4098] = 50.0                          # group 8: equal ones on both sides of a chunk's end
+    scores[36] = np.nan                                 # group 9: a score that is none
+    done[37], scores[37] = 1, np.nan
+    x[38, 17] = -1e30
+    got = _run(ctx, x, scores, beams, done)
+    _same(got, _select(x, scores, beams, done, [set()] * 40), done, beams)
+
+
+@pytest.mark.parametrize("n,window,white", [(2, 0, []), (3, 64, [5, 9]), (1, 20, []), (35, 128, [])])
+def test_selection_with_the_ngram_ban(ctx, n, window, white):
+    _say(f"ban n={n} window={window}")
+    rng = np.random.default_rng(n)
+    groups, beams, vocab, cap = 3, 4, 5000, 200
+    rows = groups * beams
+    lens = [int(v) for v in rng.integers(0, cap + 1, rows)]
+    lens[0], lens[1] = 0, cap
+    history = rng.integers(0, 12, (rows, cap)).astype(np.uint32)
+    if n == 35:
+        history[:] = np.tile(rng.integers(0, vocab, (rows, 40)), 5).astype(np.uint32)
+    x = rng.standard_normal((rows, vocab)).astype(np.float32)
+    x[:, :12] += 8  # the banned ones would win
+    banned = [_bans(history[r, :lens[r]].tolist(), n, window) - set(white) for r in range(rows)]
+    for r in range(rows):
+        for t in banned[r]:
+            x[r, t] += 3
+    scores = (-rng.random(rows)).astype(np.float32)
+    done = np.zeros(rows, np.uint8)
+    kw = dict(ngram_size=n, window=window, whitelist=ctx.to_device(np.array(white, np.uint32)) if white else None)
+    got = _run(ctx, x, scores, beams, done, history, lens, **kw)
+    assert sum(map(len, banned)) > 0
+    _same(got, _select(x, scores, beams, done, banned), done, beams)
+    with pytest.raises(_abi.ContractViolation, match="history_len"):
+        _run(ctx, x, scores, beams, done, history, [cap + 1] * rows, **kw)
+
+
+def test_selection_in_place(ctx):
+    _say("in place")
+    from franken_ocr_amd.engine import beam_select
+
+    rng = np.random.default_rng(8)
+    x = rng.standard_normal((6, 700)).astype(np.float32)
+    s, done = (-rng.random(6)).astype(np.float32), np.array([0, 1, 0, 0, 0, 1], np.uint8)
+    want = _select(x, s, 3, done, [set()] * 6)
+    ds, dd = ctx.to_device(s), ctx.to_device(done)
+    p, t = ctx.empty((6,), np.uint32), ctx.empty((6,), np.uint32)
+    beam_select(ctx.to_device(x), ds, 3, p, t, ds, done=dd, new_done=dd, eos=EOS)
+    _same((p.numpy().tolist(), t.numpy().tolist(), ds.numpy(), dd.numpy().tolist()), want, done, 3)
+
+
+def test_refusals(ctx):
+    _say("refusals")
+    from franken_ocr_amd.engine import PagedCache, RingCache, beam_reorder, beam_select
+
+    E, S = _abi.FocrHipError, _abi.ContractViolation
+    f, u = lambda *s: ctx.empty(s, np.float32), lambda *s: ctx.to_device(np.zeros(s, np.uint32))  # noqa: E731
+    for call, text in (
+            (lambda: beam_select(f(33, 10), f(33), 33, u(33), u(33), f(33)), "beams 33"),
+            (lambda: beam_select(f(4, 0), f(4), 2, u(4), u(4), f(4)), "empty logits row"),
+            (lambda: beam_select(f(4, 9), f(4), 2, u(4), u(4), f(4), ngram_size=2), "no-repeat-ngram"),
+            (lambda: beam_select(f(4, 9), f(4), 2, u(4), None, f(4)), "null"),
+            (lambda: beam_reorder(u(66), 33), "beams 33"),
+            (lambda: beam_reorder(u(4), 2, history=u(4, 8)), "history_len"),
+            (lambda: beam_reorder(u(4), 2, caches=[PagedCache(4, 16, 1, 64, ctx=ctx)]), "null"),
+            (lambda: beam_reorder(u(4), 2, caches=[PagedCache(4, 16, 1, 64, ctx=ctx), PagedCache(4, 8, 1, 64, ctx=ctx)],
+                                  tables=u(4, 2), lens=u(4)), "page sizes"),
+            (lambda: beam_reorder(u(4), 2, rings=[RingCache(3, 8, ctx=ctx)]), "3 streams"),
+            (lambda: beam_reorder(u(4), 2, rings=[RingCache(4, 8, ctx=ctx)]), "record_prefill")):
+        with pytest.raises(E, match=text):
+            call()
+    ring = RingCache(2, 8, ctx=ctx)
+    row = f(10 * 128 * 3)
+    ring.record_prefill(0, row, row, 3)
+    ring.record_prefill(1, row, row, 2)
+    with pytest.raises(_abi.StateError, match="not where its group is"):
+        beam_reorder(u(2), 2, rings=[ring])
+    beam_select(f(0, 10), f(0), 2, u(0), u(0), f(0))  # no groups: nothing to do
+    beam_reorder(u(0), 2)
+    with pytest.raises(S, match="parent"):
+        beam_reorder(ctx.to_device(np.array([0, 2], np.uint32)), 2, check=True)
+    with pytest.raises(_abi.StateError, match="history is full"):
+        beam_reorder(u(2), 2, tokens=u(2), history=u(2, 4), history_len=ctx.to_device(np.array([4, 3], np.uint32)), check=True)
+    cache = PagedCache(4, 16, 1, 64, ctx=ctx)
+    t = ctx.to_device(np.array([[0, 1], [2, 1]], np.uint32))
+    for lens, error, text in (([17, 18], _abi.StateError, "group"), ([17, 17], _abi.StateError, "another beam"),
+                              ([33, 33], _abi.StateError, "length")):
+        with pytest.raises(error, match=text):
+            beam_reorder(u(2), 2, caches=[cache], tables=t, lens=ctx.to_device(np.array(lens, np.uint32)), check=True)
+    with pytest.raises(S, match="page"):
+        beam_reorder(u(2), 2, caches=[cache], tables=ctx.to_device(np.array([[0, 1], [2, 9]], np.uint32)),
+                     lens=ctx.to_device(np.array([17, 17], np.uint32)), check=True)
+
+
+@pytest.mark.parametrize("beams,groups,layers,page,dtype", [(2, 1, 1, 16, "f32"), (5, 3, 2, 32, "bf16"), (8, 2, 3, 8, "f16"),
+                                                            (13, 1, 35, 16, "f32"), (32, 2, 1, 64, "bf16"), (1, 4, 1, 16, "f16")])
+def test_reorder_moves_the_states(ctx, beams, groups, layers, page, dtype):
+    """Histories, tables, pages in progress (also more caches than one launch takes) and rings, exactly."""
+    _say(f"reorder {groups} x {beams}, {layers} layers")
+    from franken_ocr_amd.engine import RingCache, beam_reorder
+
+    rng = np.random.default_rng(beams * 100 + layers)
+    rows, cap = groups * beams, 90
+    lens = [NONE if g == 3 else int(v) for g, v in enumerate(rng.integers(0, 5 * page, groups))]
+    if groups > 1:
+        lens[1] = 2 * page  # a page just filled
+    lens = [lens[r // beams] for r in range(rows)]
+    kv, dim = 2, 64
+    hosts = [Host(rng, ctx, lens, page, kv, dim, dtype, wide=7) for _ in range(layers)]
+    tables = hosts[0].tables.copy()
+    for h in hosts:
+        h.tables = tables
+        for name in "kv":  # what the pages hold
+            vals = rng.standard_normal(h.k.shape).astype(np.float32)
+            vals = vals.astype(np.float16).astype(np.float32) if dtype == "f16" else vals
+            if dtype == "bf16":
+                vals = ((vals.view(np.uint32) >> 16) << 16).view(np.float32)
+            setattr(h, name, vals)
+        from test_gpu_paged import _bits
+
+        h.dk.copy_from(_bits(h.k, dtype))
+        h.dv.copy_from(_bits(h.v, dtype))
+    parents = rng.integers(0, beams, rows).astype(np.uint32)
+    tokens = rng.integers(0, 1000, rows).astype(np.uint32)
+    history = rng.integers(0, 1000, (rows, cap)).astype(np.uint32)
+    sizes = np.repeat(rng.integers(0, cap, groups), beams).astype(np.uint32)
+    rings = [RingCache(rows, 16, ctx=ctx) for _ in range(2)] if rows <= 16 else []
+    held = []
+    for ring in rings:
+        parts = {}
+        for s in range(rows):
+            pk = ctx.to_device(rng.standard_normal((10, 9, 128)).astype(np.float32))
+            ring.record_prefill(s, pk, pk, 9)
+            at = ring.regions(s)
+            for name in ("ring_k", "ring_v"):
+                x = rng.standard_normal((10, 128, 128)).astype(np.float32)
+                _abi.call("focr_hip_h2d", ctx.handle, at[name], x.ctypes.data, x.nbytes)
+                parts[s, name] = x
+            ring.set_state(s, 128 if s // beams % 2 else 50, 3 if s // beams % 2 else 50)
+        held.append(parts)
+    dt, dl = ctx.to_device(tables), ctx.to_device(np.array(lens, np.uint32))
+    dh, dn = ctx.to_device(history), ctx.to_device(sizes)
+    beam_reorder(ctx.to_device(parents), beams, tokens=ctx.to_device(tokens), history=dh, history_len=dn, advance=True,
+                 caches=[h.cache for h in hosts], tables=dt, lens=dl, rings=rings, check=True)
+    src = np.arange(rows) // beams * beams + parents
+    want = history.copy()
+    for r in range(rows):
+        want[r, :sizes[r]] = history[src[r], :sizes[r]]
+        if sizes[r] < cap:
+            want[r, sizes[r]] = tokens[r]
+    assert np.array_equal(dh.numpy(), want) and np.array_equal(dn.numpy(), sizes + 1)
+    wt = tables.copy()
+    for r in range(rows):
+        if lens[r] != NONE:
+            full = lens[r] // page
+            wt[r, :full] = tables[src[r], :full]
+    assert np.array_equal(dt.numpy(), wt)
+    for h in hosts:
+        k0, v0 = h.k.copy(), h.v.copy()
+        for r in range(rows):
+            if lens[r] != NONE and lens[r] % page:
+                full, rest = lens[r] // page, lens[r] % page
+                h.k[tables[r, full], :, :rest] = k0[tables[src[r], full], :, :rest]
+                h.v[tables[r, full], :, :rest] = v0[tables[src[r], full], :, :rest]
+        h.same_pools()
+    for ring, parts in zip(rings, held):
+        for s in range(rows):
+            at = ring.regions(s)
+            count = 128 if s // beams % 2 else 50
+            for name in ("ring_k", "ring_v"):
+                x = np.empty((10, 128, 128), np.float32)
+                _abi.call("focr_hip_d2h", ctx.handle, x.ctypes.data, at[name], x.nbytes)
+                assert np.array_equal(x[:, :count], parts[src[s], name][:, :count])
+
+
+def test_reorder_without_check_leaves_what_is_no_group(ctx):
+    """Parents out of range are the slot itself; a group of different lengths keeps its tables and pages."""
+    _say("reorder, unchecked")
+    from franken_ocr_amd.engine import beam_reorder
+
+    rng = np.random.default_rng(3)
+    host = Host(rng, ctx, [20, 21, 40, 40, 40], 16, 2, 64, "f32", wide=4)
+    # a group of [20, 21] cannot be made with the third beam's length: two groups of one table each
+    parents = np.array([1, 0], np.uint32)
+    t, n = ctx.to_device(host.tables[:2]), ctx.to_device(np.array([20, 21], np.uint32))
+    beam_reorder(ctx.to_device(parents), 2, caches=[host.cache], tables=t, lens=n)
+    assert np.array_equal(t.numpy(), host.tables[:2])
+    host.same_pools()
+    t, n = ctx.to_device(host.tables[2:]), ctx.to_device(np.array([40, 40, 40], np.uint32))
+    bad = host.tables[2:].copy()
+    beam_reorder(ctx.to_device(np.array([1, 3, 0xFFFFFFFF], np.uint32)), 3, caches=[host.cache], tables=t, lens=n)
+    want = bad.copy()
+    want[0, :2] = bad[1, :2]
+    assert np.array_equal(t.numpy(), want)
+    k0, v0 = host.k.copy(), host.v.copy()
+    host.k[bad[0, 2], :, :8], host.v[bad[0, 2], :, :8] = k0[bad[1, 2], :, :8], v0[bad[1, 2], :, :8]
+    host.same_pools()
+    # a page in progress that the cache does not have: the group's pages stay
+    bad = host.tables[2:].copy()
+    bad[1, 2] = host.pages + 5
+    beam_reorder(ctx.to_device(np.array([1, 0, 0], np.uint32)), 3, caches=[host.cache], tables=ctx.to_device(bad), lens=n)
+    host.same_pools()
+
+
+def test_beam_search_over_pages_and_rings(ctx):
+    """Eight steps of search with a little model (one attention over what was read): the paged cache whose beams
+    share the prompt's pages, and the ring caches, against every beam's keys kept apart on the host in 64 bits."""
+    _say("search")
+    from franken_ocr_amd.engine import HEAD_DIM, NUM_HEADS, PagedCache, RingCache, beam_reorder, beam_select
+
+    rng = np.random.default_rng(31)
+    groups, beams, vocab, page, steps = 2, 3, 500, 16, 30
+    rows, D = groups * beams, NUM_HEADS * HEAD_DIM
+    prompts = [37, 20]
+    emb = {n: rng.standard_normal((vocab, D)).astype(np.float32) for n in "qkv"}
+    w_out = (rng.standard_normal((D, vocab)) * (6 / np.sqrt(D))).astype(np.float32)
+    wide = -(-(max(prompts) + steps + 1) // page)
+    cache = PagedCache(rows * wide, page, NUM_HEADS, HEAD_DIM, "f32", ctx=ctx)
+    tables = rng.permutation(rows * wide).astype(np.uint32).reshape(rows, wide)
+    ring = RingCache(rows, 64, ctx=ctx)
+    host = [[] for _ in range(rows)]  # each beam's (k, v) rows
+    for g in range(groups):
+        k, v = (rng.standard_normal((prompts[g], NUM_HEADS, HEAD_DIM)).astype(np.float32) for _ in "kv")
+        full = prompts[g] // page
+        for b in range(beams):
+            r = g * beams + b
+            tables[r, :full] = tables[g * beams, :full]  # the prompt's full pages are shared
+            hm = [ctx.to_device(np.ascontiguousarray(a.transpose(1, 0, 2))) for a in (k, v)]
+            ring.record_prefill(r, hm[0], hm[1], prompts[g])
+            host[r] = [(k[i], v[i]) for i in range(prompts[g])]
+        dt = ctx.to_device(tables)
+        for b in range(beams):
+            pos = np.arange(prompts[g], dtype=np.uint32)
+            if b:
+                pos[: full * page] = NONE
+            cache.write(ctx.to_device(k.reshape(-1, D)), ctx.to_device(v.reshape(-1, D)), ctx.to_device(pos), dt,
+                        seq=ctx.to_device(np.full(prompts[g], g * beams + b, np.uint32)), check=True)
+    lens = ctx.to_device(np.repeat(prompts, beams).astype(np.uint32))
+    scores = np.full(rows, -np.inf, np.float32)
+    scores[::beams] = 0.0
+    ds, dd = ctx.to_device(scores), ctx.to_device(np.zeros(rows, np.uint8))
+    history, hl = ctx.to_device(np.zeros((rows, steps), np.uint32)), ctx.to_device(np.zeros(rows, np.uint32))
+    p, t = ctx.empty((rows,), np.uint32), ctx.empty((rows,), np.uint32)
+    out, out_ring = ctx.empty((rows, D), np.float32), ctx.empty((rows, D), np.float32)
+    tokens, texts, done, mixed = np.full(rows, 2), [[] for _ in range(rows)], np.zeros(rows, np.uint8), 0
+    for i in range(steps):
+        q, k, v = (emb[n][tokens] for n in "qkv")
+        dq, dk, dv = (ctx.to_device(a) for a in (q, k, v))
+        cache.step(dq, dk, dv, dt, lens, out, advance=True)
+        ring.step(dq, dk, dv, out_ring)
+        got = out.numpy()
+        assert np.allclose(got, out_ring.numpy(), rtol=0, atol=1e-4)
+        for r in range(rows):
+            host[r] = host[r] + [(k[r].reshape(NUM_HEADS, HEAD_DIM), v[r].reshape(NUM_HEADS, HEAD_DIM))]
+            hk, hv = (np.stack([e[j] for e in host[r]]).astype(np.float64) for j in (0, 1))
+            sc = np.einsum("nhd,hd->hn", hk, q[r].reshape(NUM_HEADS, HEAD_DIM).astype(np.float64)) / np.sqrt(HEAD_DIM)
+            pr = np.exp(sc - sc.max(axis=1, keepdims=True))
+            pr /= pr.sum(axis=1, keepdims=True)
+            # scores under 60, values under 5: 2 (136 u 60 + 2^-22 + 131 u) 5 < 1e-2 at the very worst; 1e-4 of it taken
+            assert np.allclose(got[r].reshape(NUM_HEADS, HEAD_DIM), np.einsum("hn,nhd->hd", pr, hv), rtol=0, atol=1e-4)
+        logits = got @ w_out
+        now = ds.numpy()
+        banned = [_bans(texts[r], 2, 0) for r in range(rows)]
+        want = _select(logits, now, beams, done, banned)
+        beam_select(ctx.to_device(logits), ds, beams, p, t, ds, done=dd, new_done=dd, history=history, history_len=hl,
+                    ngram_size=2, window=0, eos=EOS, check=True)
+        assert p.numpy().tolist() == want[0] and t.numpy().tolist() == want[1]
+        beam_reorder(p, beams, tokens=t, history=history, history_len=hl, advance=True, caches=[cache], tables=dt, lens=lens,
+                     rings=[ring], check=True)
+        src = np.arange(rows) // beams * beams + np.array(want[0])
+        mixed += int(np.any(src != np.arange(rows)))
+        host, texts = [host[s] for s in src], [texts[s] + [x] for s, x in zip(src, want[1])]
+        tokens, done = np.array(want[1]), dd.numpy()
+        assert history.numpy()[:, : i + 1].tolist() == texts
+    assert mixed > steps // 3
+    assert lens.numpy().tolist() == np.repeat([x + steps for x in prompts], beams).tolist()
+
+
+def test_captured_beam_step_replays(ctx):
+    """Selection and reordering in one graph, replayed on changing logits, against the same calls made eagerly."""
+    _say("captured")
+    from franken_ocr_amd.device import Context
+    from franken_ocr_amd.engine import PagedCache, beam_reorder, beam_select
+
+    c = Context(0)
+    rng = np.random.default_rng(41)
+    groups, beams, vocab = 2, 4, 6000
+    rows = groups * beams
+    pool = rng.standard_normal((rows * 3, 2, 16, 64)).astype(np.float32)
+    tables = np.arange(rows * 3, dtype=np.uint32).reshape(rows, 3)
+    sides = []
+    for _ in range(2):
+        s = {"cache": PagedCache(rows * 3, 16, 2, 64, "f32", k=c.to_device(pool), v=c.to_device(pool), ctx=c),
+             "t": c.to_device(tables), "n": c.to_device(np.full(rows, 25, np.uint32)),
+             "h": c.to_device(rng.integers(0, 9, (rows, 64)).astype(np.uint32) * 0 + 3), "hl": c.to_device(np.full(rows, 10, np.uint32)),
+             "x": c.empty((rows, vocab), np.float32), "s": c.to_device(np.zeros(rows, np.float32)),
+             "p": c.empty((rows,), np.uint32), "tok": c.empty((rows,), np.uint32)}
+        sides.append(s)
+
+    def step(s):
+        beam_select(s["x"], s["s"], beams, s["p"], s["tok"], s["s"], history=s["h"], history_len=s["hl"], ngram_size=2, window=0)
+        beam_reorder(s["p"], beams, tokens=s["tok"], history=s["h"], history_len=s["hl"], advance=True, caches=[s["cache"]],
+                     tables=s["t"], lens=s["n"])
+
+    with pytest.raises(_abi.StateError, match="scratch"):
+        _capture(c, lambda: step(sides[0]))
+    x = rng.standard_normal((rows, vocab)).astype(np.float32)
+    for s in sides:
+        s["x"].copy_from(x)
+        step(s)
+    replay = _capture(c, lambda: step(sides[0]))
+    for i in range(5):
+        x = rng.standard_normal((rows, vocab)).astype(np.float32)
+        for s in sides:
+            s["x"].copy_from(x)
+        assert replay() == 0
+        c.synchronize()
+        step(sides[1])
+        for name in ("p", "tok", "s", "h", "hl", "t"):
+            assert np.array_equal(sides[0][name].numpy(), sides[1][name].numpy()), (i, name)
+        assert np.array_equal(sides[0]["cache"]._keep[0].numpy(), sides[1]["cache"]._keep[0].numpy())

@@ -1,0 +1,92 @@
+"""The paged cache's index arithmetic, walked on the host (no GPU), and the
+refusals that need no device."""
+
+from __future__ import annotations
+
+import subprocess
+from pathlib import Path
+
+import numpy as np
+import pytest
+
+ROOT = Path(__file__).resolve().parent.parent
+
+
+def test_index_arithmetic_stays_in_bounds(tmp_path):
+    exe = tmp_path / "paged_index"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", "-fsanitize=address,undefined",
+                    str(ROOT / "tests" / "paged_index.cpp"), "-o", str(exe)], check=True)
+    res = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0 and res.stdout.strip() == "ok", res.stdout + res.stderr
+
+
+class _Ctx:  # the checks below come before any call of the library
+    _h = None
+    handle = None
+
+
+def _array(shape, dtype=np.float32):
+    from franken_ocr_amd.device import DeviceArray
+
+    return DeviceArray.borrow(_Ctx(), 256, shape, dtype)
+
+
+def _cache(**kw):
+    from franken_ocr_amd.engine import PagedCache
+
+    c = PagedCache.__new__(PagedCache)
+    c.ctx, c._h = _Ctx(), None
+    c.n_pages, c.page_size, c.n_kv_heads, c.head_dim, c.dtype = 8, 16, 2, 64, "f32"
+    return c
+
+
+@pytest.mark.parametrize("change,text", [
+    ({"lens": (3,)}, "3 lengths for 4 rows"),
+    ({"q": (3, 256)}, "q of shape"),
+    ({"out": (4, 128)}, "out of shape"),
+    ({"k": (4, 64)}, "k_steps of shape"),
+    ({"prefix": (2,)}, "prefix of shape"),
+    ({"weights": (4, 3, 64)}, "weights of shape"),
+    ({"weights": (4, 128)}, "weights of shape"),
+])
+def test_step_refuses_arrays_that_do_not_fit(change, text):
+    from franken_ocr_amd import _abi
+
+    sh = {"q": (4, 256), "k": (4, 128), "v": (4, 128), "out": (4, 256), "tables": (4, 2), "lens": (4,)}
+    sh.update(change)
+    a = {n: _array(s, np.uint32 if n in ("tables", "lens", "prefix") else np.float32) for n, s in sh.items()}
+    with pytest.raises(_abi.ContractViolation, match=text):
+        _cache().step(a["q"], a["k"], a["v"], a["tables"], a["lens"], a["out"], prefix=a.get("prefix"),
+                      weights=a.get("weights"), n_heads=4)
+
+
+def test_beam_calls_refuse_rows_that_are_no_groups():
+    from franken_ocr_amd import _abi, engine
+
+    u = lambda *s: _array(s, np.uint32)  # noqa: E731
+    with pytest.raises(_abi.ContractViolation, match="no groups of 4"):
+        engine.beam_select(_array((6, 100)), _array((6,)), 4, u(6), u(6), _array((6,)))
+    with pytest.raises(_abi.ContractViolation, match="tokens of shape"):
+        engine.beam_select(_array((8, 100)), _array((8,)), 4, u(8), u(6), _array((8,)))
+    with pytest.raises(_abi.ContractViolation, match="no groups of 0"):
+        engine.beam_reorder(u(6), 0)
+    with pytest.raises(_abi.ContractViolation, match="history_len of shape"):
+        engine.beam_reorder(u(8), 4, history=u(8, 10), history_len=u(7))
+
+
+def test_unknown_dtype_is_refused():
+    from franken_ocr_amd.engine import PagedCache
+
+    with pytest.raises(ValueError, match="dtype"):
+        PagedCache(8, 16, 2, 64, "f8", ctx=_Ctx())
+
+
+def test_null_handles_are_bad_handles():
+    from franken_ocr_amd import _abi
+
+    lib = _abi.lib()
+    assert lib.focr_hip_paged_create(None, 1, 16, 1, 64, 0, None, None, None) == _abi.E_BAD_HANDLE
+    assert lib.focr_hip_paged_regions(None, None, None) == _abi.E_BAD_HANDLE
+    assert lib.focr_hip_paged_free(None) == _abi.OK
+    assert lib.focr_hip_beam_reorder(None, 1, 1, None, None, None, 0, None, 0, None, 0, None, 0, None, None, 0,
+                                     0) == _abi.E_BAD_HANDLE
