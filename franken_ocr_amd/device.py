@@ -202,7 +202,7 @@ class DeviceArray:
         return v
 
     def free(self) -> None:
-        if self._p and not getattr(self, "_borrowed", None):
+        if self._p and getattr(self, "_borrowed", None) is None:
             _abi.lib().focr_hip_dfree(self.ctx.handle, self._p)
         self._p = C.c_void_p()
 

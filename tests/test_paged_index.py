@@ -74,6 +74,25 @@ def test_beam_calls_refuse_rows_that_are_no_groups():
         engine.beam_reorder(u(8), 4, history=u(8, 10), history_len=u(7))
 
 
+@pytest.mark.parametrize("owner", [None, np.zeros(1), np.zeros(3), [], 0])
+def test_borrowed_memory_is_not_freed(monkeypatch, owner):
+    """Whatever owns it: an empty or zero owner, one without a truth value."""
+    from franken_ocr_amd import _abi
+    from franken_ocr_amd.device import DeviceArray
+
+    class Lib:
+        def focr_hip_dfree(self, *a):
+            raise AssertionError("borrowed memory freed")
+
+    monkeypatch.setattr(_abi, "lib", Lib)
+    a = DeviceArray.borrow(_Ctx(), 256, (4, 2), np.float32, owner=owner)
+    assert a.ptr == 256 and a.nbytes == 32
+    v = a.view_rows(1, 3)
+    v.free()
+    a.free()
+    assert a.ptr == 0
+
+
 def test_unknown_dtype_is_refused():
     from franken_ocr_amd.engine import PagedCache
 
