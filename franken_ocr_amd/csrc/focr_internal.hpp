@@ -749,7 +749,12 @@ struct PagedEvict {
     float* dst_weights;  // [n_seqs][n_kv_heads][dst_ldw]
     size_t dst_ldw;
     uint32_t* kept;  // [n_seqs][n_kv_heads][budget]
+    uint32_t* hist;  // paged_evict_hist_words() of workspace, null for 0
 };
+// Rows of more than a block's tile are selected by a block to a tile while
+// there are fewer of them than CUs, else by a block to a row; these words are
+// the first way's picks and histograms.
+size_t paged_evict_hist_words(size_t rows, uint32_t max_len, int cu_count);
 hipError_t launch_paged_evict(hipStream_t s, const focr_hip_paged* c, const PagedEvict& a, focr_hip_ctx* ctx);
 // Checks for calls that ask for them: err[0] = 0 where all is well, else
 // (row << 8 | code) + 1 of the first fault.
@@ -768,6 +773,7 @@ hipError_t launch_clear_words(hipStream_t s, uint32_t* p, size_t n);
 // k_beam.hip — beam search: selection over beams and vocabulary, and the
 // states of the chosen beams put where their slots are.
 constexpr int kBeamMax = 32;
+constexpr int kBeamParts = 128;  // chunks of a row at most
 struct BeamSelect {
     const float* logits;  // [groups * beams][ld]
     size_t ld;

@@ -332,11 +332,14 @@ int32_t focr_hip_paged_evict(focr_hip_ctx* ctx, focr_hip_paged* c, const uint32_
             FOCR_HIP_TRY(launch_paged_check_dst(ctx->stream, c, a, marks, k.err), "check launch");
             if ((st = k.end(who, "sequence"))) return st;
         }
+        const size_t hist = paged_evict_hist_words(n_seqs * c->n_kv_heads, a.t.max_len, ctx->cu_count);
+        const size_t words = hist + (kept ? 0 : n_seqs * c->n_kv_heads * budget);
         a.kept = kept;
-        if (!kept) {
-            a.kept = static_cast<uint32_t*>(
-                ctx->scratch_get_capturable(kScrEvict, n_seqs * c->n_kv_heads * budget * sizeof(uint32_t), who));
-            if (!a.kept) return no_scratch(ctx);
+        if (words) {
+            uint32_t* p = static_cast<uint32_t*>(ctx->scratch_get_capturable(kScrEvict, words * sizeof(uint32_t), who));
+            if (!p) return no_scratch(ctx);
+            a.hist = hist ? p : nullptr;
+            if (!kept) a.kept = p + hist;
         }
         FOCR_HIP_TRY(launch_paged_evict(ctx->stream, c, a, ctx), "paged eviction launch");
         return FOCR_HIP_OK;
@@ -356,8 +359,8 @@ int32_t focr_hip_beam_select(focr_hip_ctx* ctx, const float* logits, size_t ld, 
             return fail(FOCR_HIP_E_SHAPE, fmt("beam_select: beams %zu is outside 1 .. %d", beams, kBeamMax));
         if (vocab == 0) return fail(FOCR_HIP_E_SHAPE, "sampler::argmax_row: empty logits row");
         if (ld < vocab) return fail(FOCR_HIP_E_SHAPE, "beam_select: a row stride is shorter than the row");
-        if (vocab > (size_t(1) << 30) || groups > 65535 / beams)
-            return fail(FOCR_HIP_E_SHAPE, "beam_select: shape exceeds the gfx950 tier limit (2^30 tokens, 65535 rows)");
+        if (vocab > (size_t(1) << 19) || groups > 65535 / beams)
+            return fail(FOCR_HIP_E_SHAPE, "beam_select: shape exceeds the gfx950 tier limit (2^19 tokens, 65535 rows)");
         if (history_cap > kI32Max || ngram_size > kI32Max || window > kI32Max || n_whitelist > 4096)
             return fail(FOCR_HIP_E_SHAPE, "beam_select: history_cap / ngram_size / window / whitelist exceed the gfx950 tier limits");
         if (ngram_size && (!history || !history_len || history_cap == 0))

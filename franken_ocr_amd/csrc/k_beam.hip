@@ -19,94 +19,48 @@ namespace focr {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kPer = 16;                    // logits of a thread
-constexpr int kChunk = kThreads * kPer;     // logits of a block
+constexpr int kWaves = kThreads / 64;
+constexpr int kPer = 16;                // logits of a thread
+constexpr int kChunk = kThreads * kPer;  // logits of a block
+constexpr int kList = 128;               // candidates that a wave sorts at once
 
-// The chunks' and rows' results: max and f64 sum of exp(x - max) per chunk,
-// its W best keys (argmax_key order), then per row the sorted W best with
-// their c.
+// The chunks' results: max and f64 sum of exp(x - max) per chunk, and its W
+// best keys (argmax_key order), descending, 0 where there are fewer.
 struct Parts {
-    float* max;     // [rows][nparts]
     double* sum;    // [rows][nparts]
-    uint64_t* key;  // [rows][nparts][W], descending, 0 where there are fewer
-    double* row_c;  // [rows][W]
-    uint64_t* row_key;
+    uint64_t* key;  // [rows][nparts][W]
+    float* max;     // [rows][nparts]
 };
 
 __host__ __device__ inline Parts parts_of(void* p, int rows, int beams, int nparts) {
     Parts q;
-    const size_t n = static_cast<size_t>(rows) * nparts, w = static_cast<size_t>(rows) * beams;
+    const size_t n = static_cast<size_t>(rows) * nparts;
     q.sum = static_cast<double*>(p);
-    q.row_c = q.sum + n;
-    q.key = reinterpret_cast<uint64_t*>(q.row_c + w);
-    q.row_key = q.key + n * beams;
-    q.max = reinterpret_cast<float*>(q.row_key + w);
+    q.key = reinterpret_cast<uint64_t*>(q.sum + n);
+    q.max = reinterpret_cast<float*>(q.key + n * beams);
     return q;
 }
 
-// Grid (chunk, row): one pass over the chunk's logits, held in registers.
-__global__ __launch_bounds__(kThreads) void beam_scan_kernel(BeamSelect a, Parts q) {
-    __shared__ float s_max[kThreads / 64];
-    __shared__ double s_sum[kThreads / 64];
-    __shared__ uint64_t s_key[2][kThreads / 64];
-    const int part = blockIdx.x;
-    const int row = blockIdx.y;
-    if (a.done && a.done[row]) return;  // its one candidate needs no logits
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const float* x = a.logits + static_cast<size_t>(row) * a.ld;
-    const uint32_t* ban = a.ban_bits ? a.ban_bits + static_cast<size_t>(row) * a.ban_words : nullptr;
-    float v[kPer];
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const int t = part * kChunk + i * kThreads + static_cast<int>(threadIdx.x);
-        v[i] = t < a.vocab ? x[t] : __uint_as_float(0x7FC00000u);  // NaN: no logit
-    }
-    float m = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) m = fmaxf(m, v[i]);  // a NaN is skipped
-    m = wave_max_f_full(m);
-    if (lane == 0) s_max[wave] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
-    double sum = 0.0;
-    if (m > -INFINITY) {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const double ex = v[i] == m ? 1.0 : exp(static_cast<double>(v[i]) - static_cast<double>(m));
-            sum += v[i] == v[i] ? ex : 0.0;
-        }
-    }
-    sum = wave_sum_d_full(sum);
-    if (lane == 0) s_sum[wave] = sum;
-    uint64_t key[kPer], best = 0ull;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const int t = part * kChunk + i * kThreads + static_cast<int>(threadIdx.x);
-        key[i] = argmax_key(v[i], static_cast<uint32_t>(t));
-        if (ban && t < a.vocab && (ban[t >> 5] >> (t & 31) & 1u)) key[i] = 0ull;
-        best = umax64(best, key[i]);
-    }
-    const size_t at = static_cast<size_t>(row) * a.nparts + part;
-    for (int w = 0; w < a.beams; ++w) {
-        const uint64_t mine = wave_max_u64_full(best);
-        if (lane == 0) s_key[w & 1][wave] = mine;
-        __syncthreads();
-        const uint64_t* s = s_key[w & 1];
-        const uint64_t top = umax64(umax64(s[0], s[1]), umax64(s[2], s[3]));
-        if (threadIdx.x == 0) q.key[at * a.beams + w] = top;
-        if (top == best && top != 0ull) {  // this thread's: its next best
-            best = 0ull;
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                if (key[i] == top) key[i] = 0ull;
-                best = umax64(best, key[i]);
-            }
-        }
-    }
-    if (threadIdx.x == 0) {
-        q.max[at] = m;
-        q.sum[at] = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
-    }
+// exp(d) for d <= 0: d = n ln 2 + r with |r| <= ln 2 / 2, the Taylor series of
+// exp(r) to r^10 (its rest is below 3e-13 of the value, n's multiple of the
+// rounded ln 2 adds less), times 2^n. Below -700 as at -700, which adds
+// nothing to a sum that is at least 1.
+__device__ __forceinline__ double exp_below(double d) {
+    d = fmax(d, -700.0);
+    const double n = rint(d * 1.4426950408889634);
+    const double r = fma(n, -0.6931471805599453, d);
+    double p = 1.0 / 3628800.0;
+    p = fma(p, r, 1.0 / 362880.0);
+    p = fma(p, r, 1.0 / 40320.0);
+    p = fma(p, r, 1.0 / 5040.0);
+    p = fma(p, r, 1.0 / 720.0);
+    p = fma(p, r, 1.0 / 120.0);
+    p = fma(p, r, 1.0 / 24.0);
+    p = fma(p, r, 1.0 / 6.0);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    return ldexp(p, static_cast<int>(n));
 }
 
 // Keys of the descending list s[0..n) that are greater than k.
@@ -122,68 +76,218 @@ __device__ __forceinline__ int count_greater(const uint64_t* s, int n, uint64_t 
     return lo;
 }
 
-// Grid (row): L from the chunks, and the W best of the chunks' lists: a key's
-// place is the number of greater ones, found in every list by bisection.
-__global__ __launch_bounds__(kThreads) void beam_row_kernel(BeamSelect a, Parts q) {
-    __shared__ double s_l;
-    const int row = blockIdx.x;
-    const int W = a.beams;
-    double* rc = q.row_c + static_cast<size_t>(row) * W;
-    uint64_t* rk = q.row_key + static_cast<size_t>(row) * W;
-    const double score = static_cast<double>(a.scores[row]);
-    const bool done = a.done && a.done[row];
-    for (int i = threadIdx.x; i < W; i += kThreads) {
-        rk[i] = done && i == 0 ? (1ull << 32) | (0xFFFFFFFFull - a.eos) : 0ull;
-        rc[i] = done && i == 0 && score == score ? score : -INFINITY;
+// What lanes of this wave wrote to LDS is there for its other lanes.
+__device__ __forceinline__ void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// The W greatest of a wave's keys (a lane's are `key`), sorted, into out; 0
+// where there are fewer. A lower bound of the W-th is the W-th greatest of the
+// lanes' maxima (its leading bits, found with a ballot a bit); the few keys
+// that reach it are listed and each counts the greater ones. Where more reach
+// it than the list holds (long runs of equal logits), the maximum is taken W
+// times instead.
+__device__ __forceinline__ void wave_best(uint64_t (&key)[kPer], int W, uint64_t* list, uint64_t* out) {
+    const int lane = threadIdx.x & 63;
+    uint32_t top = 0u;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) top = max(top, static_cast<uint32_t>(key[i] >> 32));
+    uint32_t bound = 0u;
+#pragma unroll
+    for (int bit = 31; bit >= 14; --bit) {
+        const uint32_t t = bound | (1u << bit);
+        if (__popcll(__ballot(top >= t)) >= W) bound = t;
     }
-    if (done) return;
-    const size_t at = static_cast<size_t>(row) * a.nparts;
-    if (threadIdx.x < 64) {
-        float m = -INFINITY;
-        for (int p = threadIdx.x; p < a.nparts; p += 64) m = fmaxf(m, q.max[at + p]);
-        m = wave_max_f_full(m);
-        double sum = 0.0;
-        for (int p = threadIdx.x; p < a.nparts; p += 64)
-            if (q.max[at + p] > -INFINITY)
-                sum += q.sum[at + p] * (q.max[at + p] == m ? 1.0 : exp(static_cast<double>(q.max[at + p]) - static_cast<double>(m)));
-        sum = wave_sum_d_full(sum);
-        if (threadIdx.x == 0) s_l = static_cast<double>(m) + log(sum);
+    bound = max(bound, 1u);  // a key of 0 is none
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const bool in = static_cast<uint32_t>(key[i] >> 32) >= bound;
+        const uint64_t m = __ballot(in);
+        const int at = n + __popcll(m & ((1ull << lane) - 1));
+        if (in && at < kList) list[at] = key[i];
+        n += __popcll(m);
     }
-    __syncthreads();
-    const uint64_t* key = q.key + at * W;
-    for (int i = threadIdx.x; i < a.nparts * W; i += kThreads) {
-        const uint64_t k = key[i];
-        if (k == 0ull) continue;
-        int place = 0;
-        for (int p = 0; p < a.nparts && place < W; ++p) place += count_greater(key + static_cast<size_t>(p) * W, W, k);
-        if (place >= W) continue;
-        const double c = score + (static_cast<double>(key_value(k)) - s_l);
-        rk[place] = k;
-        rc[place] = c == c ? c : -INFINITY;
+    if (lane < W) out[lane] = 0ull;
+    wave_lds_fence();
+    if (n <= kList) {
+        for (int j = lane; j < n; j += 64) {
+            const uint64_t k = list[j];
+            int place = 0;
+            for (int o = 0; o < n; ++o) place += list[o] > k ? 1 : 0;
+            if (place < W) out[place] = k;
+        }
+        return;
+    }
+    uint64_t best = 0ull;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) best = umax64(best, key[i]);
+    for (int w = 0; w < W; ++w) {
+        const uint64_t k = wave_max_u64_full(best);
+        if (lane == 0) out[w] = k;
+        if (k == best) {
+            best = 0ull;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                if (key[i] == k) key[i] = 0ull;
+                best = umax64(best, key[i]);
+            }
+        }
     }
 }
 
-// Grid (group), a thread to a candidate: its place among the group's is the
-// number before it in its own beam's list and, by bisection, in the others'.
-__global__ __launch_bounds__(1024) void beam_pick_kernel(BeamSelect a, Parts q) {
+// Grid (chunk, row): one pass over the chunk's logits, held in registers.
+__global__ __launch_bounds__(kThreads) void beam_scan_kernel(BeamSelect a, Parts q) {
+    __shared__ float s_max[kWaves];
+    __shared__ double s_sum[kWaves];
+    __shared__ uint64_t s_list[kWaves][kList];
+    __shared__ uint64_t s_best[kWaves][kBeamMax];
+    const int part = blockIdx.x;
+    const int row = blockIdx.y;
+    if (a.done && a.done[row]) return;  // its one candidate needs no logits
+    const int W = a.beams;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const float* x = a.logits + static_cast<size_t>(row) * a.ld;
+    const uint32_t* ban = a.ban_bits ? a.ban_bits + static_cast<size_t>(row) * a.ban_words : nullptr;
+    float v[kPer];
+    const int t0 = part * kChunk + static_cast<int>(threadIdx.x);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) v[i] = t0 + i * kThreads < a.vocab ? x[t0 + i * kThreads] : __uint_as_float(0x7FC00000u);
+    uint32_t bw[kPer];
+    if (ban) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) bw[i] = t0 + i * kThreads < a.vocab ? ban[(t0 + i * kThreads) >> 5] : 0u;
+    }
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) m = fmaxf(m, v[i]);  // a NaN is skipped
+    m = wave_max_f_full(m);
+    // each wave sums relative to its own maximum, and they meet at the end
+    double sum = 0.0;
+    if (m > -INFINITY) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const double ex = v[i] == m ? 1.0 : exp_below(static_cast<double>(v[i]) - static_cast<double>(m));
+            sum += v[i] == v[i] ? ex : 0.0;
+        }
+    }
+    sum = wave_sum_d_full(sum);
+    if (lane == 0) {
+        s_max[wave] = m;
+        s_sum[wave] = sum;
+    }
+    uint64_t key[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        key[i] = argmax_key(v[i], static_cast<uint32_t>(t0 + i * kThreads));
+        if (ban && (bw[i] >> (t0 & 31) & 1u)) key[i] = 0ull;  // the threads' strides keep the bit's place
+    }
+    wave_best(key, W, s_list[wave], s_best[wave]);
+    __syncthreads();
+    const size_t at = static_cast<size_t>(row) * a.nparts + part;
+    if (static_cast<int>(threadIdx.x) < kWaves * W) {
+        const int w = threadIdx.x / W, j = threadIdx.x - w * W;
+        const uint64_t k = s_best[w][j];
+        int place = j, n = 0;
+#pragma unroll
+        for (int o = 0; o < kWaves; ++o) {
+            if (o != w) place += count_greater(s_best[o], W, k);
+            n += count_greater(s_best[o], W, 0ull);
+        }
+        if (k != 0ull && place < W) q.key[at * W + place] = k;
+        if (w == 0 && j >= n) q.key[at * W + j] = 0ull;
+    }
+    if (threadIdx.x == 0) {
+        float mx = s_max[0];
+        for (int o = 1; o < kWaves; ++o) mx = fmaxf(mx, s_max[o]);
+        double total = 0.0;
+        for (int o = 0; o < kWaves; ++o)
+            if (s_max[o] > -INFINITY)
+                total += s_sum[o] * (s_max[o] == mx ? 1.0 : exp_below(static_cast<double>(s_max[o]) - static_cast<double>(mx)));
+        q.max[at] = mx;
+        q.sum[at] = total;
+    }
+}
+
+// Grid (group). A wave takes a row at a time: L from the chunks, and the W
+// best keys by merging the chunks' lists, which lie in LDS (a lane has the
+// heads of its lists; the greatest goes and its list moves up). Then a thread
+// has a candidate, whose place among the group's is the number before it in
+// its own beam's list and, by bisection, in the others'.
+__global__ __launch_bounds__(1024) void beam_pick_kernel(BeamSelect a, Parts q, int waves) {
+    extern __shared__ uint64_t s_keys[];  // [waves][nparts * W]
     __shared__ double s_c[kBeamMax * kBeamMax];
     __shared__ uint64_t s_k[kBeamMax * kBeamMax];
     __shared__ int s_n[kBeamMax];  // candidates of a beam
     __shared__ uint8_t s_done[kBeamMax];
     const int W = a.beams;
     const int t = threadIdx.x;
+    const int wave = t >> 6, lane = t & 63;
     const size_t row0 = static_cast<size_t>(blockIdx.x) * W;
-    const size_t at = row0 * W;
-    if (t < W * W) {
-        s_c[t] = q.row_c[at + t];
-        s_k[t] = q.row_key[at + t];
-    }
     if (t < W) s_done[t] = a.done ? a.done[row0 + t] : 0;
+    for (int i = t; i < W * W; i += blockDim.x) s_k[i] = 0ull;
     __syncthreads();
-    if (t < W) {
+    for (int b = wave; wave < waves && b < W; b += waves) {
+        const double score = static_cast<double>(a.scores[row0 + b]);
+        if (s_done[b]) {
+            if (lane == 0) {
+                s_k[b * W] = (1ull << 32) | (0xFFFFFFFFull - a.eos);
+                s_c[b * W] = score == score ? score : -INFINITY;
+                s_n[b] = 1;
+            }
+            continue;
+        }
+        const size_t at = (row0 + b) * a.nparts;
+        uint64_t* keys = s_keys + static_cast<size_t>(wave) * a.nparts * W;
+        for (int i = lane; i < a.nparts * W; i += 64) keys[i] = q.key[at * W + i];
+        float m = -INFINITY;
+        for (int p = lane; p < a.nparts; p += 64) m = fmaxf(m, q.max[at + p]);
+        m = wave_max_f_full(m);
+        double sum = 0.0;
+        for (int p = lane; p < a.nparts; p += 64) {
+            const float mp = q.max[at + p];
+            if (mp > -INFINITY) sum += q.sum[at + p] * (mp == m ? 1.0 : exp_below(static_cast<double>(mp) - static_cast<double>(m)));
+        }
+        sum = wave_sum_d_full(sum);
+        const double total = static_cast<double>(m) + log(sum);
+        wave_lds_fence();
+        constexpr int kHeads = kBeamParts / 64;
+        uint64_t head[kHeads];
+        int next[kHeads];
+        uint64_t best = 0ull;
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) {
+            const int p = lane + 64 * h;
+            head[h] = p < a.nparts ? keys[p * W] : 0ull;
+            next[h] = p * W + 1;
+            best = umax64(best, head[h]);
+        }
         int n = 0;
-        while (n < W && s_k[t * W + n] != 0ull) ++n;
-        s_n[t] = n;
+        uint64_t mine = 0ull;  // lane w keeps the w-th best
+        for (; n < W; ++n) {
+            const uint64_t k = wave_max_u64_full(best);
+            if (k == 0ull) break;
+            if (lane == n) mine = k;
+            if (k == best) {
+                best = 0ull;
+#pragma unroll
+                for (int h = 0; h < kHeads; ++h) {
+                    if (head[h] == k) {
+                        head[h] = next[h] % W != 0 ? keys[next[h]] : 0ull;
+                        ++next[h];
+                    }
+                    best = umax64(best, head[h]);
+                }
+            }
+        }
+        if (lane < n) {
+            const double c = score + (static_cast<double>(key_value(mine)) - total);
+            s_k[b * W + lane] = mine;
+            s_c[b * W + lane] = c == c ? c : -INFINITY;
+        }
+        if (lane == 0) s_n[b] = n;
     }
     __syncthreads();
     const int b = t / W, i = t - b * W;
@@ -370,8 +474,8 @@ __global__ void beam_check_kernel(BeamReorder a, unsigned long long* err) {
 int beam_parts(int vocab) { return (vocab + kChunk - 1) / kChunk; }
 
 size_t beam_part_bytes(int rows, int beams, int nparts) {
-    const size_t n = static_cast<size_t>(rows) * nparts, w = static_cast<size_t>(rows) * beams;
-    return n * 8 + w * 8 + n * beams * 8 + w * 8 + n * 4;
+    const size_t n = static_cast<size_t>(rows) * nparts;
+    return n * (sizeof(double) + sizeof(float) + beams * sizeof(uint64_t));
 }
 
 hipError_t launch_beam_select(hipStream_t s, const BeamSelect& a, focr_hip_ctx* ctx) {
@@ -379,9 +483,12 @@ hipError_t launch_beam_select(hipStream_t s, const BeamSelect& a, focr_hip_ctx* 
     const Parts q = parts_of(a.part, rows, a.beams, a.nparts);
     ProfScope ps(ctx, "beam_select");
     FOCR_LAUNCH(beam_scan_kernel, dim3(a.nparts, rows), dim3(kThreads), 0, s, a, q);
-    FOCR_LAUNCH(beam_row_kernel, dim3(rows), dim3(kThreads), 0, s, a, q);
-    const int t = (a.beams * a.beams + 63) / 64 * 64;
-    FOCR_LAUNCH(beam_pick_kernel, dim3(a.groups), dim3(t), 0, s, a, q);
+    // a row's lists in LDS for as many rows at once as 128 KB hold (one: nparts * beams <= 4096 keys, 32 KB)
+    const size_t row_bytes = static_cast<size_t>(a.nparts) * a.beams * sizeof(uint64_t);
+    const int waves = static_cast<int>(std::min<size_t>({16, static_cast<size_t>(a.beams), (size_t(128) << 10) / row_bytes}));
+    const size_t lds = waves * row_bytes;
+    const int threads = std::max(64 * waves, (a.beams * a.beams + 63) / 64 * 64);
+    FOCR_LAUNCH(beam_pick_kernel, dim3(a.groups), dim3(threads), lds, s, a, q, waves);
     return hipGetLastError();
 }
 

@@ -129,6 +129,27 @@ __device__ __forceinline__ float fold_lanes(float v, Op op) {
     return v;
 }
 
+// The four waves' maxima, sums and outputs of GT heads joined and written as
+// split z's part; row0: the first head's row of all [sequence][head].
+template <int GT, int D>
+__device__ __forceinline__ void join_waves(const PagedAttend& a, const float (*s_acc)[GT][D], const float2 (*s_ml)[GT],
+                                           int g0, size_t row0, int z) {
+    for (int at = threadIdx.x; at < GT * D; at += 256) {
+        const int i = at / D, d = at - i * D;
+        if (g0 + i >= a.group) break;
+        const float m0 = s_ml[0][i].x, m1 = s_ml[1][i].x, m2 = s_ml[2][i].x, m3 = s_ml[3][i].x;
+        const float mx = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+        const float sf = mx == -INFINITY ? 0.0f : mx;
+        const float w0 = __builtin_amdgcn_exp2f(m0 - sf), w1 = __builtin_amdgcn_exp2f(m1 - sf);
+        const float w2 = __builtin_amdgcn_exp2f(m2 - sf), w3 = __builtin_amdgcn_exp2f(m3 - sf);
+        const float o = s_acc[0][i][d] * w0 + s_acc[1][i][d] * w1 + s_acc[2][i][d] * w2 + s_acc[3][i][d] * w3;
+        const size_t part = (row0 + i) * a.nsplit + z;
+        a.part_acc[part * D + d] = o;
+        if (d == 0)
+            a.part_ml[part] = make_float2(mx, s_ml[0][i].y * w0 + s_ml[1][i].y * w1 + s_ml[2][i].y * w2 + s_ml[3][i].y * w3);
+    }
+}
+
 // One split of one key head's keys, for GT of its query heads. Grid (split,
 // key head x head tile, sequence), 4 waves. Every wave takes tiles of its own:
 // C lanes hold a key's row (16 bytes each), 64 / C keys to a load
@@ -294,20 +315,194 @@ __global__ __launch_bounds__(256) void paged_attend_kernel(PoolGeom g, PagedAtte
             for (int j = 0; j < E; ++j) s_acc[wave][i][cl * E + j] = acc[i][j];
     }
     __syncthreads();
-    for (int at = threadIdx.x; at < GT * D; at += 256) {
-        const int i = at / D, d = at - i * D;
-        if (g0 + i >= a.group) break;
-        const float m0 = s_ml[0][i].x, m1 = s_ml[1][i].x, m2 = s_ml[2][i].x, m3 = s_ml[3][i].x;
-        const float mx = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
-        const float sf = mx == -INFINITY ? 0.0f : mx;
-        const float w0 = __builtin_amdgcn_exp2f(m0 - sf), w1 = __builtin_amdgcn_exp2f(m1 - sf);
-        const float w2 = __builtin_amdgcn_exp2f(m2 - sf), w3 = __builtin_amdgcn_exp2f(m3 - sf);
-        const float o = s_acc[0][i][d] * w0 + s_acc[1][i][d] * w1 + s_acc[2][i][d] * w2 + s_acc[3][i][d] * w3;
-        const size_t part = (static_cast<size_t>(s) * n_heads + head0 + i) * a.nsplit + z;
-        a.part_acc[part * D + d] = o;
-        if (d == 0)
-            a.part_ml[part] = make_float2(mx, s_ml[0][i].y * w0 + s_ml[1][i].y * w1 + s_ml[2][i].y * w2 + s_ml[3][i].y * w3);
+    join_waves<GT, D>(a, s_acc, s_ml, g0, head0 + static_cast<size_t>(s) * n_heads, z);
+}
+
+// The same split on the f32 matrix cores, for up to 16 query heads of a key
+// head at once (grid (split, key head x tile of 16 heads, sequence)). A wave
+// takes 16 keys at a time on v_mfma_f32_16x16x4_f32, lane l = 16 a + b:
+//   scores  S[key][head]: A = K (lane: key b, one of the row's 16-byte pieces
+//           a + 4 c), B = q (lane: head b, the same values of d). The result
+//           leaves lane l with head b and the keys 4 a + i, i < 4 ...
+//   output  O[head][d]: ... which is what A of step i takes (head b, key
+//           4 a + i), so the probabilities stay where they are; B = V (lane:
+//           key 4 a + i, pieces b + 16 c of its row, one value at a time).
+// The running maximum is moved only where a score is more than 2^8 times past
+// it (any reference gives the same quotient, and f32 holds the sums), so the
+// usual tile needs nothing from other lanes.
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+
+template <typename T, int D>
+__global__ __launch_bounds__(256) void paged_attend_mfma_kernel(PoolGeom g, PagedAttend a) {
+    constexpr int E = Row16<T>::N;
+    constexpr int C = D / E;                   // 16-byte pieces of a row
+    constexpr int KC = C / 4;                  // K pieces of a lane
+    constexpr int VE = C >= 16 ? E : E / 2;    // values of a V piece (8 bytes where a row has 8 pieces of 16)
+    constexpr int VC = D / (16 * VE);          // V pieces of a lane and key
+    constexpr int VD = VC * VE;                // output columns of a lane
+    __shared__ uint32_t s_row[kPagedChunkMax];
+    __shared__ float s_acc[4][16][D];
+    __shared__ float2 s_ml[4][16];
+    const int z = blockIdx.x;
+    const int tiles = (a.group + 15) / 16;
+    const int hk = blockIdx.y / tiles;
+    const int g0 = (blockIdx.y - hk * tiles) * 16;
+    const int s = blockIdx.z;
+    const Seen e = seen_of(a.t, a.prefix, a.window, a.k_steps != nullptr, s);
+    if (z == 0 && blockIdx.y == 0 && threadIdx.x == 0)
+        a.seen[s] = make_uint4(e.none ? kPagedNone : e.nvis, e.p, e.shift, e.own ? 1u : 0u);
+    if (e.none) return;
+    const uint32_t chunk = split_keys(e.nvis, a.nsplit);
+    const uint32_t b0 = static_cast<uint32_t>(z) * chunk;
+    if (b0 >= e.nvis) return;
+    const int cnt = static_cast<int>(min(chunk, e.nvis - b0));
+    const int padded = (cnt + 15) & ~15;
+    for (int j = threadIdx.x; j < padded; j += 256) {
+        const uint32_t at = b0 + j;
+        s_row[j] = j < cnt ? row_of(a.t, g, s, hk, at < e.p ? at : at + e.shift) : kBadRow;
     }
+    const int wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63;
+    const int la = lane >> 4;
+    const int lb = lane & 15;
+    const bool head = g0 + lb < a.group;
+    const size_t head0 = static_cast<size_t>(hk) * a.group + g0;
+    const size_t n_heads = static_cast<size_t>(g.kv_heads) * a.group;
+    float q[KC][E];
+    {
+        const float* qr = a.q + static_cast<size_t>(s) * a.ldq + (head0 + lb) * D + la * E;
+        const float qscale = a.scale * kLog2e;
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+#pragma unroll
+            for (int j = 0; j < E; ++j) q[c][j] = head ? qr[4 * E * c + j] * qscale : 0.0f;
+    }
+    const int own = e.own && e.nvis - 1 - b0 < static_cast<uint32_t>(cnt) ? static_cast<int>(e.nvis - 1 - b0) : -1;
+    float m = -INFINITY, l = 0.0f;  // of head lb, this lane's keys
+    v4f acc[VC][VE];                // of heads 4 la + r, columns (lb + 16 c) VE + j
+#pragma unroll
+    for (int c = 0; c < VC; ++c)
+#pragma unroll
+        for (int j = 0; j < VE; ++j) acc[c][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    __syncthreads();
+    for (int t0 = wave * 16; t0 < cnt; t0 += 64) {
+        const uint32_t krow = s_row[t0 + lb];
+        const uint4 vrow4 = *reinterpret_cast<const uint4*>(s_row + t0 + 4 * la);
+        const uint32_t vrow[4] = {vrow4.x, vrow4.y, vrow4.z, vrow4.w};
+        u4 kw[KC];
+        u4 vw[4][VC];
+        const u4* kp = static_cast<const u4*>(g.k) + la;
+        const auto vload = [&](uint32_t row, int c) -> u4 {
+            const char* p = static_cast<const char*>(g.v) + (static_cast<size_t>(row) * D + (lb + 16 * c) * VE) * sizeof(T);
+            if constexpr (VE * sizeof(T) == 8) {
+                const u2 w = *reinterpret_cast<const u2*>(p);
+                return u4{w[0], w[1], 0, 0};
+            } else {
+                return *reinterpret_cast<const u4*>(p);
+            }
+        };
+        if (__all(krow != kBadRow)) {
+#pragma unroll
+            for (int c = 0; c < KC; ++c) kw[c] = kp[static_cast<size_t>(krow) * C + 4 * c];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int c = 0; c < VC; ++c) vw[i][c] = vload(vrow[i], c);
+        } else {  // slots that hold no key are not read: what lies there may be NaN
+#pragma unroll
+            for (int c = 0; c < KC; ++c) kw[c] = krow != kBadRow ? kp[static_cast<size_t>(krow) * C + 4 * c] : u4{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int c = 0; c < VC; ++c) vw[i][c] = vrow[i] != kBadRow ? vload(vrow[i], c) : u4{0, 0, 0, 0};
+        }
+        if (own >= t0 && own < t0 + 16) {  // the step's row comes from the call and goes to its page
+            const size_t at = static_cast<size_t>(s) * a.ldkv + static_cast<size_t>(hk) * D;
+            float f[8];
+            if (t0 + lb == own && krow != kBadRow) {
+#pragma unroll
+                for (int c = 0; c < KC; ++c) {
+#pragma unroll
+                    for (int j = 0; j < E; ++j) f[j] = a.k_steps[at + (la + 4 * c) * E + j];
+                    kw[c] = Row16<T>::pack(f);
+                    if (g0 == 0) static_cast<u4*>(g.k)[static_cast<size_t>(krow) * C + la + 4 * c] = kw[c];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (t0 + 4 * la + i == own && vrow[i] != kBadRow) {
+#pragma unroll
+                    for (int c = 0; c < VC; ++c) {
+#pragma unroll
+                        for (int j = 0; j < E; ++j) f[j] = j < VE ? a.v_steps[at + (lb + 16 * c) * VE + j] : 0.0f;
+                        vw[i][c] = Row16<T>::pack(f);
+                        if (g0 == 0) {
+                            char* p = static_cast<char*>(g.v) + (static_cast<size_t>(vrow[i]) * D + (lb + 16 * c) * VE) * sizeof(T);
+                            if constexpr (VE * sizeof(T) == 8)
+                                *reinterpret_cast<u2*>(p) = u2{vw[i][c][0], vw[i][c][1]};
+                            else
+                                *reinterpret_cast<u4*>(p) = vw[i][c];
+                        }
+                    }
+                }
+            }
+        }
+        v4f sc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+            float f[E];
+            Row16<T>::load(kw[c], f);
+#pragma unroll
+            for (int j = 0; j < E; ++j) sc = __builtin_amdgcn_mfma_f32_16x16x4f32(f[j], q[c][j], sc, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[i] = vrow[i] != kBadRow ? sc[i] : -INFINITY;
+        if (a.scores && head) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (t0 + 4 * la + i < cnt)
+                    a.scores[(static_cast<size_t>(s) * n_heads + head0 + lb) * a.score_ld + b0 + t0 + 4 * la + i] = sc[i];
+        }
+        float mx = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
+        if (__any(mx > m + 8.0f)) {
+            mx = fmaxf(fold_lanes<16, 64>(mx, Max()), m);
+            const float corr = __builtin_amdgcn_exp2f(m - (mx == -INFINITY ? 0.0f : mx));
+            m = mx;
+            l *= corr;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float cr = __shfl(corr, 4 * la + r, 64);
+#pragma unroll
+                for (int c = 0; c < VC; ++c)
+#pragma unroll
+                    for (int j = 0; j < VE; ++j) acc[c][j][r] *= cr;
+            }
+        }
+        const float safe = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float p = __builtin_amdgcn_exp2f(sc[i] - safe);
+            l += p;
+#pragma unroll
+            for (int c = 0; c < VC; ++c) {
+                float f[E];
+                Row16<T>::load(vw[i][c], f);
+#pragma unroll
+                for (int j = 0; j < VE; ++j) acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(p, f[j], acc[c][j], 0, 0, 0);
+            }
+        }
+    }
+    l = fold_lanes<16, 64>(l, Sum());
+    if (lane < 16) s_ml[wave][lane] = make_float2(m, l);
+#pragma unroll
+    for (int c = 0; c < VC; ++c)
+#pragma unroll
+        for (int j = 0; j < VE; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s_acc[wave][4 * la + r][(lb + 16 * c) * VE + j] = acc[c][j][r];
+    __syncthreads();
+    join_waves<16, D>(a, s_acc, s_ml, g0, head0 + static_cast<size_t>(s) * n_heads, z);
 }
 
 // Grid (head, sequence): the splits of a row joined, out = sum_z acc_z f_z /
@@ -442,93 +637,251 @@ __device__ __forceinline__ uint32_t weight_key(float v) {
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// Grid (key head, sequence): the threshold by four passes over 8 bits of the
-// keys each (a histogram of the keys that share the bits found so far), then
-// the slots that stay in order: those above the threshold, and of those at it
-// the first ones.
-__global__ __launch_bounds__(1024) void paged_select_kernel(PagedEvict a, uint32_t kv_heads) {
-    __shared__ uint32_t s_hist[256];
-    __shared__ uint32_t s_pick[2];  // the digit, and how many are wanted within it
-    __shared__ uint32_t s_above[16], s_equal[16];
+// The threshold is found by digits of 11, 11 and 10 bits of the keys, from the
+// top: a histogram of the keys that share the digits found so far, then the
+// digit in whose bin the last of the wanted ones falls.
+constexpr int kBins = 2048;
+constexpr int kSelThreads = 1024;
+constexpr int kSelWaves = kSelThreads / 64;
+constexpr int kDigitShift[3] = {21, 10, 0};
+
+struct Pick {
+    uint32_t found, want;  // the digits so far; how many of the keys that share them stay
+};
+
+// Bins from the top until `want` keys are counted; hist in LDS or registers:
+// thread t holds the counts of bins 2047 - 2 t and 2046 - 2 t.
+__device__ __forceinline__ Pick find_digit(uint32_t hi, uint32_t lo, Pick p, int shift, uint32_t* s_wave, Pick* s_pick) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const uint32_t sum = hi + lo;
+    uint32_t incl = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t v = __shfl_up(incl, o, 64);
+        incl += lane >= o ? v : 0u;
+    }
+    if (lane == 63) s_wave[wave] = incl;
+    __syncthreads();
+    uint32_t before = incl - sum;
+#pragma unroll
+    for (int i = 0; i < kSelWaves; ++i) before += i < wave ? s_wave[i] : 0u;
+    if (before < p.want && p.want - before <= sum) {
+        const uint32_t bin = kBins - 1 - 2 * threadIdx.x;
+        const bool up = p.want - before <= hi;
+        s_pick->found = p.found | ((up ? bin : bin - 1) << shift);
+        s_pick->want = p.want - before - (up ? 0u : hi);
+    }
+    __syncthreads();
+    return *s_pick;
+}
+
+// A thread's keys of a tile of kSelThreads * KPT slots: slot (wave KPT + i) 64
+// + lane of the tile, so that the slots of a wave follow each other.
+template <int KPT>
+struct SelTile {
+    float v[KPT];
+    uint32_t j0;
+    __device__ __forceinline__ uint32_t slot(int i) const { return j0 + i * 64; }
+    __device__ __forceinline__ void load(const float* w, const Cut& c, uint32_t tile) {
+        j0 = tile * (kSelThreads * KPT) + (threadIdx.x >> 6) * (KPT * 64) + (threadIdx.x & 63);
+#pragma unroll
+        for (int i = 0; i < KPT; ++i) v[i] = slot(i) < c.n ? w[slot(i)] : 0.0f;
+    }
+    __device__ __forceinline__ bool middle(const Cut& c, int i) const { return slot(i) >= c.lo && slot(i) < c.hi; }
+    __device__ __forceinline__ void count(const Cut& c, uint32_t found, int pass, uint32_t* s_hist) const {
+        const int shift = kDigitShift[pass];
+        const uint32_t mask = pass == 2 ? 1023u : kBins - 1u;
+        const int known = pass == 0 ? 32 : kDigitShift[pass - 1];
+#pragma unroll
+        for (int i = 0; i < KPT; ++i) {
+            const uint32_t k = weight_key(v[i]);
+            if (middle(c, i) && (pass == 0 || (k >> known) == (found >> known))) atomicAdd(&s_hist[(k >> shift) & mask], 1u);
+        }
+    }
+    // The slots that stay, in order, behind `above` slots above the threshold
+    // and `equal` at it; advances both by the tile's.
+    __device__ __forceinline__ void place(const Cut& c, Pick t, uint32_t& above, uint32_t& equal, uint32_t (*s_n)[kSelWaves],
+                                          uint32_t* kept, float* dw) const {
+        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+        const uint64_t below = (1ull << lane) - 1;
+        uint32_t na = 0, ne = 0;
+#pragma unroll
+        for (int i = 0; i < KPT; ++i) {
+            na += __popcll(__ballot(is_above(c, t, i)));
+            ne += __popcll(__ballot(is_equal(c, t, i)));
+        }
+        if (lane == 0) {
+            s_n[0][wave] = na;
+            s_n[1][wave] = ne;
+        }
+        __syncthreads();
+        uint32_t wa = above, we = equal;
+#pragma unroll
+        for (int i = 0; i < kSelWaves; ++i) {
+            wa += i < wave ? s_n[0][i] : 0u;
+            we += i < wave ? s_n[1][i] : 0u;
+            above += s_n[0][i];
+            equal += s_n[1][i];
+        }
+#pragma unroll
+        for (int i = 0; i < KPT; ++i) {
+            const bool up = is_above(c, t, i), eq = is_equal(c, t, i);
+            const uint64_t ma = __ballot(up), me = __ballot(eq);
+            const uint32_t e0 = we + __popcll(me & below);  // equal ones before this slot
+            if (up || (eq && e0 < t.want)) {
+                const uint32_t to = wa + __popcll(ma & below) + min(e0, t.want);
+                kept[to] = slot(i);
+                dw[to] = v[i];
+            }
+            wa += __popcll(ma);
+            we += __popcll(me);
+        }
+        __syncthreads();
+    }
+    __device__ __forceinline__ bool is_above(const Cut& c, Pick t, int i) const {
+        return slot(i) < c.n && (c.whole || !middle(c, i) || (t.want != 0u && weight_key(v[i]) > t.found));
+    }
+    __device__ __forceinline__ bool is_equal(const Cut& c, Pick t, int i) const {
+        return !c.whole && t.want != 0u && middle(c, i) && weight_key(v[i]) == t.found;
+    }
+};
+
+// Grid (key head, sequence): a row of weights by one block, in registers where
+// it fits a tile (read once), else a tile at a time in every pass.
+template <int KPT>
+__global__ __launch_bounds__(kSelThreads) void paged_select_kernel(PagedEvict a, uint32_t kv_heads) {
+    __shared__ uint32_t s_hist[kBins];
+    __shared__ uint32_t s_n[2][kSelWaves];
+    __shared__ Pick s_pick;
     const int hk = blockIdx.x;
     const int s = blockIdx.y;
     const Cut c = cut_of(a, s);
-    if (hk == 0 && threadIdx.x == 0) a.dst_lens[s] = c.none ? kPagedNone : min(c.n, a.budget);
     if (c.none) return;
     const size_t row = static_cast<size_t>(s) * kv_heads + hk;
     const float* w = a.weights + row * a.ldw;
-    uint32_t* kept = a.kept + row * a.budget;
-    float* dw = a.dst_weights + row * a.dst_ldw;
-    if (c.whole) {
-        for (uint32_t j = threadIdx.x; j < c.n; j += 1024) {
-            kept[j] = j;
-            dw[j] = w[j];
-        }
-        return;
-    }
-    uint32_t found = 0, want = c.want;  // the threshold's bits so far; how many of the keys that share them stay
-    for (int shift = 24; shift >= 0 && want; shift -= 8) {
-        if (threadIdx.x < 256) s_hist[threadIdx.x] = 0;
-        __syncthreads();
-        for (uint32_t j = c.lo + threadIdx.x; j < c.hi; j += 1024) {
-            const uint32_t k = weight_key(w[j]);
-            if (shift == 24 || (k >> (shift + 8)) == (found >> (shift + 8))) atomicAdd(&s_hist[(k >> shift) & 255u], 1u);
-        }
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            uint32_t left = want;
-            int b = 255;
-            for (; b > 0 && s_hist[b] < left; --b) left -= s_hist[b];
-            s_pick[0] = static_cast<uint32_t>(b);
-            s_pick[1] = left;
-        }
-        __syncthreads();
-        found |= s_pick[0] << shift;
-        want = s_pick[1];
-    }
-    // want: how many at the threshold stay (0: none is wanted at all)
-    const bool any = c.want != 0;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    uint32_t base = 0, equal_base = 0;
-    for (uint32_t j0 = 0; j0 < c.n; j0 += 1024) {
-        const uint32_t j = j0 + threadIdx.x;
-        const float v = j < c.n ? w[j] : 0.0f;
-        const bool middle = j >= c.lo && j < c.hi;
-        const uint32_t k = weight_key(v);
-        const bool above = j < c.n && (!middle || (any && k > found));
-        const bool equal = any && middle && k == found;
-        const uint64_t ma = __ballot(above), me = __ballot(equal);
-        if (lane == 0) {
-            s_above[wave] = __popcll(ma);
-            s_equal[wave] = __popcll(me);
-        }
-        __syncthreads();
-        uint32_t wa = 0, we = 0, ta = 0, te = 0;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            if (i < wave) {
-                wa += s_above[i];
-                we += s_equal[i];
+    const uint32_t tiles = (c.n + kSelThreads * KPT - 1) / (kSelThreads * KPT);
+    SelTile<KPT> t;
+    t.load(w, c, 0);
+    Pick p{0u, c.want};
+    if (!c.whole && c.want != 0) {
+        for (int pass = 0; pass < 3; ++pass) {
+            s_hist[threadIdx.x] = s_hist[threadIdx.x + kSelThreads] = 0u;
+            __syncthreads();
+            for (uint32_t i = 0; i < tiles; ++i) {
+                if (tiles > 1) t.load(w, c, i);
+                t.count(c, p.found, pass, s_hist);
             }
-            ta += s_above[i];
-            te += s_equal[i];
+            __syncthreads();
+            p = find_digit(s_hist[kBins - 1 - 2 * threadIdx.x], s_hist[kBins - 2 - 2 * threadIdx.x], p, kDigitShift[pass], s_n[0], &s_pick);
         }
-        const uint64_t below = (1ull << lane) - 1;
-        const uint32_t e0 = equal_base + we + __popcll(me & below);  // equal ones before this slot
-        const bool stay = above || (equal && e0 < want);
-        if (stay) {
-            const uint32_t to = base + wa + __popcll(ma & below) + (min(e0, want) - min(equal_base, want));
-            kept[to] = j;
-            dw[to] = v;
-        }
-        base += ta + (min(equal_base + te, want) - min(equal_base, want));
-        equal_base += te;
-        __syncthreads();
+    }
+    uint32_t above = 0, equal = 0;
+    for (uint32_t i = 0; i < tiles; ++i) {
+        if (tiles > 1) t.load(w, c, i);
+        t.place(c, p, above, equal, s_n, a.kept + row * a.budget, a.dst_weights + row * a.dst_ldw);
     }
 }
 
+// The same for few long rows: a block to a tile of a row, a launch to a pass.
+// Every block writes its histogram to [row][tile][pass]; the next launch's
+// blocks each add up their row's and find its digit again.
+constexpr int kLongKpt = 16;
+constexpr uint32_t kLongTile = kSelThreads * kLongKpt;
+
+__device__ __forceinline__ Pick long_digit(const uint32_t* hist, uint32_t tiles, int pass, Pick p, uint32_t* s_wave, Pick* s_pick) {
+    uint32_t hi = 0, lo = 0;
+    for (uint32_t i = 0; i < tiles; ++i) {
+        const uint32_t* h = hist + (static_cast<size_t>(i) * 3 + pass) * kBins + (kBins - 2 - 2 * threadIdx.x);
+        lo += h[0];
+        hi += h[1];
+    }
+    return find_digit(hi, lo, p, kDigitShift[pass], s_wave, s_pick);
+}
+
+__global__ __launch_bounds__(kSelThreads) void paged_hist_kernel(PagedEvict a, uint32_t kv_heads, uint32_t* hist, Pick* picks,
+                                                                 int pass) {
+    __shared__ uint32_t s_hist[kBins];
+    __shared__ uint32_t s_wave[kSelWaves];
+    __shared__ Pick s_pick;
+    const uint32_t tile = blockIdx.x;
+    const int s = blockIdx.z;
+    const Cut c = cut_of(a, s);
+    if (c.none || c.whole || c.want == 0 || tile * kLongTile >= c.n) return;
+    const size_t row = static_cast<size_t>(s) * kv_heads + blockIdx.y;
+    const uint32_t tiles = (c.n + kLongTile - 1) / kLongTile;
+    uint32_t* rh = hist + row * gridDim.x * 3 * kBins;
+    SelTile<kLongKpt> t;
+    t.load(a.weights + row * a.ldw, c, tile);
+    Pick p{0u, c.want};
+    if (pass > 0) {
+        if (pass > 1) p = picks[row * 2];
+        p = long_digit(rh, tiles, pass - 1, p, s_wave, &s_pick);
+        if (tile == 0 && threadIdx.x == 0) picks[row * 2 + pass - 1] = p;
+    }
+    s_hist[threadIdx.x] = s_hist[threadIdx.x + kSelThreads] = 0u;
+    __syncthreads();
+    t.count(c, p.found, pass, s_hist);
+    __syncthreads();
+    uint32_t* to = rh + (static_cast<size_t>(tile) * 3 + pass) * kBins;
+    to[threadIdx.x] = s_hist[threadIdx.x];
+    to[threadIdx.x + kSelThreads] = s_hist[threadIdx.x + kSelThreads];
+}
+
+__global__ __launch_bounds__(kSelThreads) void paged_place_kernel(PagedEvict a, uint32_t kv_heads, const uint32_t* hist,
+                                                                  const Pick* picks) {
+    __shared__ uint32_t s_n[2][kSelWaves];
+    __shared__ Pick s_pick;
+    const uint32_t tile = blockIdx.x;
+    const int s = blockIdx.z;
+    const Cut c = cut_of(a, s);
+    if (c.none || tile * kLongTile >= c.n) return;
+    const size_t row = static_cast<size_t>(s) * kv_heads + blockIdx.y;
+    SelTile<kLongKpt> t;
+    t.load(a.weights + row * a.ldw, c, tile);
+    const uint32_t tiles = (c.n + kLongTile - 1) / kLongTile;
+    const uint32_t* rh = hist + row * gridDim.x * 3 * kBins;
+    Pick p{0u, c.want};
+    uint32_t above = 0, equal = 0;
+    if (!c.whole && c.want != 0) {
+        p = long_digit(rh, tiles, 2, picks[row * 2 + 1], s_n[0], &s_pick);
+        // what the tiles before this one hold: above in a digit's bins past the found one, at the last digit's own bin
+        uint32_t na = 0, ne = 0;
+        for (uint32_t i = 0; i < tile; ++i) {
+#pragma unroll
+            for (int pass = 0; pass < 3; ++pass) {
+                const uint32_t digit = (p.found >> kDigitShift[pass]) & (pass == 2 ? 1023u : kBins - 1u);
+                const uint32_t* h = rh + (static_cast<size_t>(i) * 3 + pass) * kBins;
+                for (uint32_t b = threadIdx.x; b < kBins; b += kSelThreads) {
+                    const uint32_t n = h[b];
+                    na += b > digit ? n : 0u;
+                    ne += pass == 2 && b == digit ? n : 0u;
+                }
+            }
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            na += __shfl_xor(na, o, 64);
+            ne += __shfl_xor(ne, o, 64);
+        }
+        if ((threadIdx.x & 63) == 0) {
+            s_n[0][threadIdx.x >> 6] = na;
+            s_n[1][threadIdx.x >> 6] = ne;
+        }
+        __syncthreads();
+        for (int i = 0; i < kSelWaves; ++i) {
+            above += s_n[0][i];
+            equal += s_n[1][i];
+        }
+        __syncthreads();
+    }
+    const uint32_t first = tile * kLongTile;  // and the slots before it that stay anyway
+    above += c.whole ? first : min(first, c.lo) + (first > c.hi ? first - c.hi : 0u);
+    t.place(c, p, above, equal, s_n, a.kept + row * a.budget, a.dst_weights + row * a.dst_ldw);
+}
+
 // Grid (tile of kept slots, key head, sequence): their rows into the pages of
-// dst_tables, 16 bytes a lane.
+// dst_tables, 16 bytes a lane. The new lengths are written here: dst_lens may
+// be lens, and min(length, budget) is the same of the old and the new.
 template <int C>
 __global__ __launch_bounds__(256) void paged_gather_kernel(PoolGeom g, PagedEvict a) {
     constexpr int R = 256 / C;  // rows a step
@@ -536,10 +889,10 @@ __global__ __launch_bounds__(256) void paged_gather_kernel(PoolGeom g, PagedEvic
     const int hk = blockIdx.y;
     const int s = blockIdx.z;
     const uint32_t len = a.t.lens[s];
-    if (len == kPagedNone) return;
     const uint32_t n = min(min(len, a.t.max_len), a.budget);
+    if (blockIdx.x == 0 && hk == 0 && threadIdx.x == 0) a.dst_lens[s] = len == kPagedNone ? kPagedNone : n;
     const uint32_t i0 = blockIdx.x * (R * U);
-    if (i0 >= n) return;
+    if (len == kPagedNone || i0 >= n) return;
     const int cl = threadIdx.x % C;
     const uint32_t* kept = a.kept + (static_cast<size_t>(s) * g.kv_heads + hk) * a.budget;
     const PagedTables dst{a.dst_tables, nullptr, a.t.n_seqs, a.dst_max_pages, 0};
@@ -657,7 +1010,7 @@ void attend(hipStream_t s, const focr_hip_paged* c, const PagedAttend& a) {
     else if (a.group <= 4)
         FOCR_LAUNCH((paged_attend_kernel<T, D, 4, 4>), grid(4), dim3(256), 0, s, g, a);
     else
-        FOCR_LAUNCH((paged_attend_kernel<T, D, 8, 4>), grid(8), dim3(256), 0, s, g, a);
+        FOCR_LAUNCH((paged_attend_mfma_kernel<T, D>), grid(16), dim3(256), 0, s, g, a);
 }
 
 template <typename T>
@@ -724,11 +1077,30 @@ hipError_t launch_paged_write(hipStream_t s, const focr_hip_paged* c, const floa
     return hipGetLastError();
 }
 
+size_t paged_evict_hist_words(size_t rows, uint32_t max_len, int cu_count) {
+    const size_t tiles = (static_cast<size_t>(max_len) + kLongTile - 1) / kLongTile;
+    return tiles > 1 && rows < static_cast<size_t>(cu_count) ? rows * (4 + tiles * 3 * kBins) : 0;
+}
+
 hipError_t launch_paged_evict(hipStream_t s, const focr_hip_paged* c, const PagedEvict& a, focr_hip_ctx* ctx) {
     const PoolGeom g = geom_of(c);
     {
         ProfScope ps(ctx, "paged_select");
-        FOCR_LAUNCH(paged_select_kernel, dim3(g.kv_heads, a.t.n_seqs), dim3(1024), 0, s, a, g.kv_heads);
+        const dim3 rows(g.kv_heads, a.t.n_seqs), block(kSelThreads);
+        if (a.hist) {
+            const dim3 grid((a.t.max_len + kLongTile - 1) / kLongTile, g.kv_heads, a.t.n_seqs);
+            Pick* picks = reinterpret_cast<Pick*>(a.hist);
+            uint32_t* hist = a.hist + 4 * static_cast<size_t>(a.t.n_seqs) * g.kv_heads;
+            for (int pass = 0; pass < 3; ++pass)
+                FOCR_LAUNCH(paged_hist_kernel, grid, block, 0, s, a, g.kv_heads, hist, picks, pass);
+            FOCR_LAUNCH(paged_place_kernel, grid, block, 0, s, a, g.kv_heads, hist, picks);
+        } else if (a.t.max_len <= 2 * kSelThreads) {
+            FOCR_LAUNCH(paged_select_kernel<2>, rows, block, 0, s, a, g.kv_heads);
+        } else if (a.t.max_len <= 8 * kSelThreads) {
+            FOCR_LAUNCH(paged_select_kernel<8>, rows, block, 0, s, a, g.kv_heads);
+        } else {
+            FOCR_LAUNCH(paged_select_kernel<kLongKpt>, rows, block, 0, s, a, g.kv_heads);
+        }
     }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -736,7 +1108,7 @@ hipError_t launch_paged_evict(hipStream_t s, const focr_hip_paged* c, const Page
     const uint32_t most = std::min(a.budget, a.t.max_len);
     const int lanes = static_cast<int>(c->head_dim * c->esize() / 16);
     const uint32_t rows = 4 * (256 / lanes);
-    const dim3 grid((most + rows - 1) / rows, g.kv_heads, a.t.n_seqs);
+    const dim3 grid(std::max<uint32_t>((most + rows - 1) / rows, 1), g.kv_heads, a.t.n_seqs);
     if (lanes == 8)
         FOCR_LAUNCH(paged_gather_kernel<8>, grid, dim3(256), 0, s, g, a);
     else if (lanes == 16)

@@ -67,7 +67,7 @@ FOCR_INDEX uint32_t split_keys(uint32_t nvis, int nsplit) {
 // most kPagedChunkMax keys (their rows are kept in LDS) and of at least
 // kPagedChunkUnit.
 inline int pick_splits(size_t n_seqs, size_t kv_heads, int group, uint32_t max_seen, int cu_count) {
-    const size_t tiles = static_cast<size_t>((group + 7) / 8);
+    const size_t tiles = static_cast<size_t>((group + 15) / 16);
     const size_t base = std::max<size_t>(n_seqs * kv_heads * tiles, 1);
     const size_t least = (static_cast<size_t>(max_seen) + kPagedChunkMax - 1) / kPagedChunkMax;
     const size_t most = (static_cast<size_t>(max_seen) + kPagedChunkUnit - 1) / kPagedChunkUnit;

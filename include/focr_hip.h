@@ -508,7 +508,7 @@ int32_t focr_hip_paged_evict(focr_hip_ctx* ctx, focr_hip_paged* cache, const uin
 
 /* ---- beam search -----------------------------------------------------------
  * No counterpart in the reference (its sampler is greedy). Row g * beams + b
- * is beam b of group g; beams <= 32. */
+ * is beam b of group g; beams <= 32, vocab <= 524288. */
 /* One step's selection over logits [groups * beams][vocab] (rows ld apart) and
  * scores [groups * beams] (log probabilities; -inf for a beam that is not
  * there, as all but one of a group at its start): the candidates are score +
