@@ -22,7 +22,7 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kPer = 16;                // logits of a thread
 constexpr int kChunk = kThreads * kPer;  // logits of a block
-constexpr int kList = 128;               // candidates that a wave sorts at once
+constexpr int kList = 256;               // candidates of a chunk that are sorted at once
 
 // The chunks' results: max and f64 sum of exp(x - max) per chunk, and its W
 // best keys (argmax_key order), descending, 0 where there are fewer.
@@ -63,19 +63,6 @@ __device__ __forceinline__ double exp_below(double d) {
     return ldexp(p, static_cast<int>(n));
 }
 
-// Keys of the descending list s[0..n) that are greater than k.
-__device__ __forceinline__ int count_greater(const uint64_t* s, int n, uint64_t k) {
-    int lo = 0, hi = n;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (s[mid] > k)
-            lo = mid + 1;
-        else
-            hi = mid;
-    }
-    return lo;
-}
-
 // What lanes of this wave wrote to LDS is there for its other lanes.
 __device__ __forceinline__ void wave_lds_fence() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -83,67 +70,34 @@ __device__ __forceinline__ void wave_lds_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// The W greatest of a wave's keys (a lane's are `key`), sorted, into out; 0
-// where there are fewer. A lower bound of the W-th is the W-th greatest of the
-// lanes' maxima (its leading bits, found with a ballot a bit); the few keys
-// that reach it are listed and each counts the greater ones. Where more reach
-// it than the list holds (long runs of equal logits), the maximum is taken W
-// times instead.
-__device__ __forceinline__ void wave_best(uint64_t (&key)[kPer], int W, uint64_t* list, uint64_t* out) {
-    const int lane = threadIdx.x & 63;
-    uint32_t top = 0u;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) top = max(top, static_cast<uint32_t>(key[i] >> 32));
+// A float's place in the order of floats, as a whole number (NaN: 0), -0 as +0.
+__device__ __forceinline__ uint32_t float_order(float v) { return static_cast<uint32_t>(argmax_key(v, 0u) >> 32); }
+
+// A number that at least W of a wave's lanes reach with theirs: the leading
+// bits of the W-th greatest, a ballot a bit; 0 where fewer than W have one.
+__device__ __forceinline__ uint32_t wave_bound(uint32_t mine, int W) {
     uint32_t bound = 0u;
 #pragma unroll
-    for (int bit = 31; bit >= 14; --bit) {
+    for (int bit = 31; bit >= 12; --bit) {
         const uint32_t t = bound | (1u << bit);
-        if (__popcll(__ballot(top >= t)) >= W) bound = t;
+        if (__popcll(__ballot(mine >= t)) >= W) bound = t;
     }
-    bound = max(bound, 1u);  // a key of 0 is none
-    int n = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const bool in = static_cast<uint32_t>(key[i] >> 32) >= bound;
-        const uint64_t m = __ballot(in);
-        const int at = n + __popcll(m & ((1ull << lane) - 1));
-        if (in && at < kList) list[at] = key[i];
-        n += __popcll(m);
-    }
-    if (lane < W) out[lane] = 0ull;
-    wave_lds_fence();
-    if (n <= kList) {
-        for (int j = lane; j < n; j += 64) {
-            const uint64_t k = list[j];
-            int place = 0;
-            for (int o = 0; o < n; ++o) place += list[o] > k ? 1 : 0;
-            if (place < W) out[place] = k;
-        }
-        return;
-    }
-    uint64_t best = 0ull;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) best = umax64(best, key[i]);
-    for (int w = 0; w < W; ++w) {
-        const uint64_t k = wave_max_u64_full(best);
-        if (lane == 0) out[w] = k;
-        if (k == best) {
-            best = 0ull;
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                if (key[i] == k) key[i] = 0ull;
-                best = umax64(best, key[i]);
-            }
-        }
-    }
+    return bound;
 }
 
-// Grid (chunk, row): one pass over the chunk's logits, held in registers.
+// Grid (chunk, row): one pass over the chunk's logits, held in registers. Its W
+// best: at least W of a wave's lanes have a logit that reaches the wave's
+// bound, so only logits that reach the greatest of the four waves' bounds can
+// be among them. They are few; they are listed and each counts the greater
+// ones. Where the list does not hold them (long runs of equal logits), the
+// maximum is taken W times instead.
 __global__ __launch_bounds__(kThreads) void beam_scan_kernel(BeamSelect a, Parts q) {
     __shared__ float s_max[kWaves];
     __shared__ double s_sum[kWaves];
-    __shared__ uint64_t s_list[kWaves][kList];
-    __shared__ uint64_t s_best[kWaves][kBeamMax];
+    __shared__ uint32_t s_bound[kWaves];
+    __shared__ uint64_t s_list[kList];
+    __shared__ uint64_t s_key[2][kWaves];
+    __shared__ int s_n;
     const int part = blockIdx.x;
     const int row = blockIdx.y;
     if (a.done && a.done[row]) return;  // its one candidate needs no logits
@@ -151,63 +105,118 @@ __global__ __launch_bounds__(kThreads) void beam_scan_kernel(BeamSelect a, Parts
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const float* x = a.logits + static_cast<size_t>(row) * a.ld;
     const uint32_t* ban = a.ban_bits ? a.ban_bits + static_cast<size_t>(row) * a.ban_words : nullptr;
+    const float none = __uint_as_float(0x7FC00000u);  // NaN: no logit
     float v[kPer];
     const int t0 = part * kChunk + static_cast<int>(threadIdx.x);
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) v[i] = t0 + i * kThreads < a.vocab ? x[t0 + i * kThreads] : __uint_as_float(0x7FC00000u);
-    uint32_t bw[kPer];
+    for (int i = 0; i < kPer; ++i) v[i] = t0 + i * kThreads < a.vocab ? x[t0 + i * kThreads] : none;
+    uint32_t banned = 0u;  // bit i: v[i] is
     if (ban) {
+        uint32_t bw[kPer];
 #pragma unroll
         for (int i = 0; i < kPer; ++i) bw[i] = t0 + i * kThreads < a.vocab ? ban[(t0 + i * kThreads) >> 5] : 0u;
-    }
-    float m = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) m = fmaxf(m, v[i]);  // a NaN is skipped
-    m = wave_max_f_full(m);
-    // each wave sums relative to its own maximum, and they meet at the end
+        for (int i = 0; i < kPer; ++i) banned |= (bw[i] >> (t0 & 31) & 1u) << i;  // kThreads keeps the bit's place
+    }
+    if (threadIdx.x == 0) s_n = 0;
+    float most = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) most = fmaxf(most, v[i]);  // a NaN is skipped
+    const float m = wave_max_f_full(most);
+    // each wave sums relative to its own maximum, and they meet at the end; a
+    // NaN's difference counts as -700, which adds nothing beside the maximum's 1
     double sum = 0.0;
     if (m > -INFINITY) {
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            const double ex = v[i] == m ? 1.0 : exp_below(static_cast<double>(v[i]) - static_cast<double>(m));
-            sum += v[i] == v[i] ? ex : 0.0;
+            const double d = static_cast<double>(v[i]) - static_cast<double>(m);
+            sum += exp_below(v[i] == m ? 0.0 : d);
         }
     }
     sum = wave_sum_d_full(sum);
+    if (__any(banned)) {
+        most = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            v[i] = banned >> i & 1u ? none : v[i];
+            most = fmaxf(most, v[i]);
+        }
+    }
+    // a lane without a logit above -inf counts as having none for the bound alone
+    const uint32_t bound = wave_bound(most > -INFINITY ? float_order(most) : 0u, W);
     if (lane == 0) {
         s_max[wave] = m;
         s_sum[wave] = sum;
+        s_bound[wave] = bound;
     }
-    uint64_t key[kPer];
+    __syncthreads();
+    const uint32_t top = max(max(s_bound[0], s_bound[1]), max(s_bound[2], s_bound[3]));
+    const float least = top ? key_value(static_cast<uint64_t>(top) << 32) : -INFINITY;
+    int n = 0;
+    uint64_t in[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        key[i] = argmax_key(v[i], static_cast<uint32_t>(t0 + i * kThreads));
-        if (ban && (bw[i] >> (t0 & 31) & 1u)) key[i] = 0ull;  // the threads' strides keep the bit's place
+        in[i] = __ballot(v[i] >= least);
+        n += __popcll(in[i]);
     }
-    wave_best(key, W, s_list[wave], s_best[wave]);
-    __syncthreads();
-    const size_t at = static_cast<size_t>(row) * a.nparts + part;
-    if (static_cast<int>(threadIdx.x) < kWaves * W) {
-        const int w = threadIdx.x / W, j = threadIdx.x - w * W;
-        const uint64_t k = s_best[w][j];
-        int place = j, n = 0;
+    int at = 0;
+    if (n) {
+        if (lane == 0) at = atomicAdd(&s_n, n);
+        at = __builtin_amdgcn_readfirstlane(at);
 #pragma unroll
-        for (int o = 0; o < kWaves; ++o) {
-            if (o != w) place += count_greater(s_best[o], W, k);
-            n += count_greater(s_best[o], W, 0ull);
+        for (int i = 0; i < kPer; ++i) {
+            if (in[i]) {
+                const int to = at + __popcll(in[i] & ((1ull << lane) - 1));
+                if ((in[i] >> lane & 1u) && to < kList) s_list[to] = argmax_key(v[i], static_cast<uint32_t>(t0 + i * kThreads));
+                at += __popcll(in[i]);
+            }
         }
-        if (k != 0ull && place < W) q.key[at * W + place] = k;
-        if (w == 0 && j >= n) q.key[at * W + j] = 0ull;
+    }
+    __syncthreads();
+    n = s_n;
+    const size_t to = static_cast<size_t>(row) * a.nparts + part;
+    uint64_t* out = q.key + to * W;
+    if (n <= kList) {
+        for (int j = threadIdx.x; j < n; j += kThreads) {
+            const uint64_t k = s_list[j];
+            int place = 0;
+#pragma unroll 8
+            for (int o = 0; o < n; ++o) place += s_list[o] > k ? 1 : 0;
+            if (place < W) out[place] = k;
+        }
+        for (int j = n + threadIdx.x; j < W; j += kThreads) out[j] = 0ull;
+    } else {
+        uint64_t key[kPer], best = 0ull;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            key[i] = argmax_key(v[i], static_cast<uint32_t>(t0 + i * kThreads));
+            best = umax64(best, key[i]);
+        }
+        for (int w = 0; w < W; ++w) {
+            const uint64_t mine = wave_max_u64_full(best);
+            if (lane == 0) s_key[w & 1][wave] = mine;
+            __syncthreads();
+            const uint64_t* k = s_key[w & 1];
+            const uint64_t now = umax64(umax64(k[0], k[1]), umax64(k[2], k[3]));
+            if (threadIdx.x == 0) out[w] = now;
+            if (now == best) {
+                best = 0ull;
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) {
+                    if (key[i] == now) key[i] = 0ull;
+                    best = umax64(best, key[i]);
+                }
+            }
+        }
     }
     if (threadIdx.x == 0) {
-        float mx = s_max[0];
-        for (int o = 1; o < kWaves; ++o) mx = fmaxf(mx, s_max[o]);
+        const float mx = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
         double total = 0.0;
         for (int o = 0; o < kWaves; ++o)
             if (s_max[o] > -INFINITY)
-                total += s_sum[o] * (s_max[o] == mx ? 1.0 : exp_below(static_cast<double>(s_max[o]) - static_cast<double>(mx)));
-        q.max[at] = mx;
-        q.sum[at] = total;
+                total += s_sum[o] * exp_below(s_max[o] == mx ? 0.0 : static_cast<double>(s_max[o]) - static_cast<double>(mx));
+        q.max[to] = mx;
+        q.sum[to] = total;
     }
 }
 
@@ -248,7 +257,7 @@ __global__ __launch_bounds__(1024) void beam_pick_kernel(BeamSelect a, Parts q, 
         double sum = 0.0;
         for (int p = lane; p < a.nparts; p += 64) {
             const float mp = q.max[at + p];
-            if (mp > -INFINITY) sum += q.sum[at + p] * (mp == m ? 1.0 : exp_below(static_cast<double>(mp) - static_cast<double>(m)));
+            if (mp > -INFINITY) sum += q.sum[at + p] * exp_below(mp == m ? 0.0 : static_cast<double>(mp) - static_cast<double>(m));
         }
         sum = wave_sum_d_full(sum);
         const double total = static_cast<double>(m) + log(sum);

@@ -386,37 +386,49 @@ __global__ __launch_bounds__(256) void paged_attend_mfma_kernel(PoolGeom g, Page
 #pragma unroll
         for (int j = 0; j < VE; ++j) acc[c][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     __syncthreads();
-    for (int t0 = wave * 16; t0 < cnt; t0 += 64) {
-        const uint32_t krow = s_row[t0 + lb];
+    struct Tile {
+        uint32_t krow, vrow[4];
+        u4 kw[KC], vw[4][VC];
+    };
+    const u4* kp = static_cast<const u4*>(g.k) + la;
+    const auto vload = [&](uint32_t row, int c) -> u4 {
+        const char* p = static_cast<const char*>(g.v) + (static_cast<size_t>(row) * D + (lb + 16 * c) * VE) * sizeof(T);
+        if constexpr (VE * sizeof(T) == 8) {
+            const u2 w = *reinterpret_cast<const u2*>(p);
+            return u4{w[0], w[1], 0, 0};
+        } else {
+            return *reinterpret_cast<const u4*>(p);
+        }
+    };
+    const auto fetch = [&](Tile& t, int t0) {
+        t.krow = s_row[t0 + lb];
         const uint4 vrow4 = *reinterpret_cast<const uint4*>(s_row + t0 + 4 * la);
-        const uint32_t vrow[4] = {vrow4.x, vrow4.y, vrow4.z, vrow4.w};
-        u4 kw[KC];
-        u4 vw[4][VC];
-        const u4* kp = static_cast<const u4*>(g.k) + la;
-        const auto vload = [&](uint32_t row, int c) -> u4 {
-            const char* p = static_cast<const char*>(g.v) + (static_cast<size_t>(row) * D + (lb + 16 * c) * VE) * sizeof(T);
-            if constexpr (VE * sizeof(T) == 8) {
-                const u2 w = *reinterpret_cast<const u2*>(p);
-                return u4{w[0], w[1], 0, 0};
-            } else {
-                return *reinterpret_cast<const u4*>(p);
-            }
-        };
-        if (__all(krow != kBadRow)) {
+        t.vrow[0] = vrow4.x;
+        t.vrow[1] = vrow4.y;
+        t.vrow[2] = vrow4.z;
+        t.vrow[3] = vrow4.w;
+        if (__all(t.krow != kBadRow)) {
 #pragma unroll
-            for (int c = 0; c < KC; ++c) kw[c] = kp[static_cast<size_t>(krow) * C + 4 * c];
+            for (int c = 0; c < KC; ++c) t.kw[c] = kp[static_cast<size_t>(t.krow) * C + 4 * c];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int c = 0; c < VC; ++c) vw[i][c] = vload(vrow[i], c);
+                for (int c = 0; c < VC; ++c) t.vw[i][c] = vload(t.vrow[i], c);
         } else {  // slots that hold no key are not read: what lies there may be NaN
 #pragma unroll
-            for (int c = 0; c < KC; ++c) kw[c] = krow != kBadRow ? kp[static_cast<size_t>(krow) * C + 4 * c] : u4{0, 0, 0, 0};
+            for (int c = 0; c < KC; ++c)
+                t.kw[c] = t.krow != kBadRow ? kp[static_cast<size_t>(t.krow) * C + 4 * c] : u4{0, 0, 0, 0};
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int c = 0; c < VC; ++c) vw[i][c] = vrow[i] != kBadRow ? vload(vrow[i], c) : u4{0, 0, 0, 0};
+                for (int c = 0; c < VC; ++c) t.vw[i][c] = t.vrow[i] != kBadRow ? vload(t.vrow[i], c) : u4{0, 0, 0, 0};
         }
+    };
+    const auto attend = [&](Tile& t, int t0) {
+        uint32_t (&vrow)[4] = t.vrow;
+        const uint32_t krow = t.krow;
+        u4 (&kw)[KC] = t.kw;
+        u4 (&vw)[4][VC] = t.vw;
         if (own >= t0 && own < t0 + 16) {  // the step's row comes from the call and goes to its page
             const size_t at = static_cast<size_t>(s) * a.ldkv + static_cast<size_t>(hk) * D;
             float f[8];
@@ -492,6 +504,11 @@ __global__ __launch_bounds__(256) void paged_attend_mfma_kernel(PoolGeom g, Page
                 for (int j = 0; j < VE; ++j) acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(p, f[j], acc[c][j], 0, 0, 0);
             }
         }
+    };
+    for (int t0 = wave * 16; t0 < cnt; t0 += 64) {
+        Tile t;
+        fetch(t, t0);
+        attend(t, t0);
     }
     l = fold_lanes<16, 64>(l, Sum());
     if (lane < 16) s_ml[wave][lane] = make_float2(m, l);
@@ -785,23 +802,65 @@ __global__ __launch_bounds__(kSelThreads) void paged_select_kernel(PagedEvict a,
 // The same for few long rows: a block to a tile of a row, a launch to a pass.
 // Every block writes its histogram to [row][tile][pass]; the next launch's
 // blocks each add up their row's and find its digit again.
-constexpr int kLongKpt = 16;
+constexpr int kLongKpt = 8;
 constexpr uint32_t kLongTile = kSelThreads * kLongKpt;
 
-__device__ __forceinline__ Pick long_digit(const uint32_t* hist, uint32_t tiles, int pass, Pick p, uint32_t* s_wave, Pick* s_pick) {
-    uint32_t hi = 0, lo = 0;
+// The digit of a pass from the row's histograms, and in `above` how many keys of
+// this block's tile (own) or of the tiles before it lie past the digit, in
+// `at` how many at it.
+__device__ __forceinline__ Pick long_digit(const uint32_t* hist, uint32_t tiles, uint32_t tile, bool own, int pass, Pick p,
+                                           uint32_t* s_wave, Pick* s_pick, uint32_t& above, uint32_t& at) {
+    uint32_t hi = 0, lo = 0, mine_hi = 0, mine_lo = 0;
+    const uint32_t* h = hist + static_cast<size_t>(pass) * kBins + (kBins - 2 - 2 * threadIdx.x);
+#pragma unroll 8
     for (uint32_t i = 0; i < tiles; ++i) {
-        const uint32_t* h = hist + (static_cast<size_t>(i) * 3 + pass) * kBins + (kBins - 2 - 2 * threadIdx.x);
-        lo += h[0];
-        hi += h[1];
+        const uint2 n = *reinterpret_cast<const uint2*>(h + static_cast<size_t>(i) * 3 * kBins);
+        const bool m = own ? i == tile : i < tile;
+        lo += n.x;
+        hi += n.y;
+        mine_lo += m ? n.x : 0u;
+        mine_hi += m ? n.y : 0u;
     }
-    return find_digit(hi, lo, p, kDigitShift[pass], s_wave, s_pick);
+    p = find_digit(hi, lo, p, kDigitShift[pass], s_wave, s_pick);
+    const uint32_t digit = (p.found >> kDigitShift[pass]) & (pass == 2 ? 1023u : kBins - 1u);
+    const uint32_t bin = kBins - 1 - 2 * threadIdx.x;
+    above = (bin > digit ? mine_hi : 0u) + (bin - 1 > digit ? mine_lo : 0u);
+    at = bin == digit ? mine_hi : bin - 1 == digit ? mine_lo : 0u;
+    return p;
 }
 
-__global__ __launch_bounds__(kSelThreads) void paged_hist_kernel(PagedEvict a, uint32_t kv_heads, uint32_t* hist, Pick* picks,
-                                                                 int pass) {
+// The block's sums of two counts, in every thread.
+__device__ __forceinline__ void block_sum2(uint32_t& x, uint32_t& y, uint32_t (*s_n)[kSelWaves]) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        x += __shfl_xor(x, o, 64);
+        y += __shfl_xor(y, o, 64);
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) {
+        s_n[0][threadIdx.x >> 6] = x;
+        s_n[1][threadIdx.x >> 6] = y;
+    }
+    __syncthreads();
+    x = y = 0;
+#pragma unroll
+    for (int i = 0; i < kSelWaves; ++i) {
+        x += s_n[0][i];
+        y += s_n[1][i];
+    }
+    __syncthreads();
+}
+
+// counts [row][tile][2]: the keys of a tile past the first and second digit.
+struct LongRows {
+    Pick* picks;       // [rows][2]
+    uint32_t* counts;  // [rows][tiles][2]
+    uint32_t* hist;    // [rows][tiles][3][kBins]
+};
+
+__global__ __launch_bounds__(kSelThreads) void paged_hist_kernel(PagedEvict a, uint32_t kv_heads, LongRows r, int pass) {
     __shared__ uint32_t s_hist[kBins];
-    __shared__ uint32_t s_wave[kSelWaves];
+    __shared__ uint32_t s_n[2][kSelWaves];
     __shared__ Pick s_pick;
     const uint32_t tile = blockIdx.x;
     const int s = blockIdx.z;
@@ -809,16 +868,21 @@ __global__ __launch_bounds__(kSelThreads) void paged_hist_kernel(PagedEvict a, u
     if (c.none || c.whole || c.want == 0 || tile * kLongTile >= c.n) return;
     const size_t row = static_cast<size_t>(s) * kv_heads + blockIdx.y;
     const uint32_t tiles = (c.n + kLongTile - 1) / kLongTile;
-    uint32_t* rh = hist + row * gridDim.x * 3 * kBins;
+    uint32_t* rh = r.hist + row * gridDim.x * 3 * kBins;
     SelTile<kLongKpt> t;
     t.load(a.weights + row * a.ldw, c, tile);
+    s_hist[threadIdx.x] = s_hist[threadIdx.x + kSelThreads] = 0u;
     Pick p{0u, c.want};
     if (pass > 0) {
-        if (pass > 1) p = picks[row * 2];
-        p = long_digit(rh, tiles, pass - 1, p, s_wave, &s_pick);
-        if (tile == 0 && threadIdx.x == 0) picks[row * 2 + pass - 1] = p;
+        if (pass > 1) p = r.picks[row * 2];
+        uint32_t above, at;
+        p = long_digit(rh, tiles, tile, true, pass - 1, p, s_n[0], &s_pick, above, at);
+        block_sum2(above, at, s_n);
+        if (threadIdx.x == 0) {
+            r.counts[(row * gridDim.x + tile) * 2 + pass - 1] = above;
+            if (tile == 0) r.picks[row * 2 + pass - 1] = p;
+        }
     }
-    s_hist[threadIdx.x] = s_hist[threadIdx.x + kSelThreads] = 0u;
     __syncthreads();
     t.count(c, p.found, pass, s_hist);
     __syncthreads();
@@ -827,8 +891,7 @@ __global__ __launch_bounds__(kSelThreads) void paged_hist_kernel(PagedEvict a, u
     to[threadIdx.x + kSelThreads] = s_hist[threadIdx.x + kSelThreads];
 }
 
-__global__ __launch_bounds__(kSelThreads) void paged_place_kernel(PagedEvict a, uint32_t kv_heads, const uint32_t* hist,
-                                                                  const Pick* picks) {
+__global__ __launch_bounds__(kSelThreads) void paged_place_kernel(PagedEvict a, uint32_t kv_heads, LongRows r) {
     __shared__ uint32_t s_n[2][kSelWaves];
     __shared__ Pick s_pick;
     const uint32_t tile = blockIdx.x;
@@ -839,40 +902,12 @@ __global__ __launch_bounds__(kSelThreads) void paged_place_kernel(PagedEvict a, 
     SelTile<kLongKpt> t;
     t.load(a.weights + row * a.ldw, c, tile);
     const uint32_t tiles = (c.n + kLongTile - 1) / kLongTile;
-    const uint32_t* rh = hist + row * gridDim.x * 3 * kBins;
     Pick p{0u, c.want};
     uint32_t above = 0, equal = 0;
     if (!c.whole && c.want != 0) {
-        p = long_digit(rh, tiles, 2, picks[row * 2 + 1], s_n[0], &s_pick);
-        // what the tiles before this one hold: above in a digit's bins past the found one, at the last digit's own bin
-        uint32_t na = 0, ne = 0;
-        for (uint32_t i = 0; i < tile; ++i) {
-#pragma unroll
-            for (int pass = 0; pass < 3; ++pass) {
-                const uint32_t digit = (p.found >> kDigitShift[pass]) & (pass == 2 ? 1023u : kBins - 1u);
-                const uint32_t* h = rh + (static_cast<size_t>(i) * 3 + pass) * kBins;
-                for (uint32_t b = threadIdx.x; b < kBins; b += kSelThreads) {
-                    const uint32_t n = h[b];
-                    na += b > digit ? n : 0u;
-                    ne += pass == 2 && b == digit ? n : 0u;
-                }
-            }
-        }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            na += __shfl_xor(na, o, 64);
-            ne += __shfl_xor(ne, o, 64);
-        }
-        if ((threadIdx.x & 63) == 0) {
-            s_n[0][threadIdx.x >> 6] = na;
-            s_n[1][threadIdx.x >> 6] = ne;
-        }
-        __syncthreads();
-        for (int i = 0; i < kSelWaves; ++i) {
-            above += s_n[0][i];
-            equal += s_n[1][i];
-        }
-        __syncthreads();
+        p = long_digit(r.hist + row * gridDim.x * 3 * kBins, tiles, tile, false, 2, r.picks[row * 2 + 1], s_n[0], &s_pick, above, equal);
+        for (uint32_t i = threadIdx.x; i < 2 * tile; i += kSelThreads) above += r.counts[row * gridDim.x * 2 + i];
+        block_sum2(above, equal, s_n);
     }
     const uint32_t first = tile * kLongTile;  // and the slots before it that stay anyway
     above += c.whole ? first : min(first, c.lo) + (first > c.hi ? first - c.hi : 0u);
@@ -1079,7 +1114,7 @@ hipError_t launch_paged_write(hipStream_t s, const focr_hip_paged* c, const floa
 
 size_t paged_evict_hist_words(size_t rows, uint32_t max_len, int cu_count) {
     const size_t tiles = (static_cast<size_t>(max_len) + kLongTile - 1) / kLongTile;
-    return tiles > 1 && rows < static_cast<size_t>(cu_count) ? rows * (4 + tiles * 3 * kBins) : 0;
+    return tiles > 1 && rows < static_cast<size_t>(cu_count) ? rows * (4 + tiles * (2 + 3 * kBins)) : 0;
 }
 
 hipError_t launch_paged_evict(hipStream_t s, const focr_hip_paged* c, const PagedEvict& a, focr_hip_ctx* ctx) {
@@ -1089,17 +1124,16 @@ hipError_t launch_paged_evict(hipStream_t s, const focr_hip_paged* c, const Page
         const dim3 rows(g.kv_heads, a.t.n_seqs), block(kSelThreads);
         if (a.hist) {
             const dim3 grid((a.t.max_len + kLongTile - 1) / kLongTile, g.kv_heads, a.t.n_seqs);
-            Pick* picks = reinterpret_cast<Pick*>(a.hist);
-            uint32_t* hist = a.hist + 4 * static_cast<size_t>(a.t.n_seqs) * g.kv_heads;
-            for (int pass = 0; pass < 3; ++pass)
-                FOCR_LAUNCH(paged_hist_kernel, grid, block, 0, s, a, g.kv_heads, hist, picks, pass);
-            FOCR_LAUNCH(paged_place_kernel, grid, block, 0, s, a, g.kv_heads, hist, picks);
+            const size_t n = static_cast<size_t>(a.t.n_seqs) * g.kv_heads;
+            const LongRows r{reinterpret_cast<Pick*>(a.hist), a.hist + 4 * n, a.hist + 4 * n + 2 * n * grid.x};
+            for (int pass = 0; pass < 3; ++pass) FOCR_LAUNCH(paged_hist_kernel, grid, block, 0, s, a, g.kv_heads, r, pass);
+            FOCR_LAUNCH(paged_place_kernel, grid, block, 0, s, a, g.kv_heads, r);
         } else if (a.t.max_len <= 2 * kSelThreads) {
             FOCR_LAUNCH(paged_select_kernel<2>, rows, block, 0, s, a, g.kv_heads);
         } else if (a.t.max_len <= 8 * kSelThreads) {
             FOCR_LAUNCH(paged_select_kernel<8>, rows, block, 0, s, a, g.kv_heads);
         } else {
-            FOCR_LAUNCH(paged_select_kernel<kLongKpt>, rows, block, 0, s, a, g.kv_heads);
+            FOCR_LAUNCH(paged_select_kernel<16>, rows, block, 0, s, a, g.kv_heads);
         }
     }
     hipError_t e = hipGetLastError();

@@ -71,7 +71,7 @@ inline int pick_splits(size_t n_seqs, size_t kv_heads, int group, uint32_t max_s
     const size_t base = std::max<size_t>(n_seqs * kv_heads * tiles, 1);
     const size_t least = (static_cast<size_t>(max_seen) + kPagedChunkMax - 1) / kPagedChunkMax;
     const size_t most = (static_cast<size_t>(max_seen) + kPagedChunkUnit - 1) / kPagedChunkUnit;
-    const size_t fill = (8 * static_cast<size_t>(cu_count) + base - 1) / base;
+    const size_t fill = (6 * static_cast<size_t>(cu_count) + base - 1) / base;
     return static_cast<int>(std::max<size_t>(std::min(std::max(fill, least), most), 1));
 }
 
