@@ -698,7 +698,7 @@ hipError_t launch_rswa_attention(hipStream_t s, const focr_hip_rswa* c, size_t s
 
 // k_paged.hip — the paged cache. Row r of the tables is sequence r's pages.
 constexpr uint32_t kPagedNone = 0xFFFFFFFFu;  // lens[s]: no sequence in this row
-constexpr int kPagedChunkMax = 2048;          // keys of one split
+constexpr int kPagedChunkMax = 512;           // keys of one split
 constexpr int kPagedChunkUnit = 64;           // splits are whole multiples of this
 struct PagedTables {
     const uint32_t* tables;  // [n_seqs][max_pages]
@@ -723,7 +723,8 @@ struct PagedAttend {
     size_t ldo;
     float* weights;  // [n_seqs][n_kv_heads][ldw], nullable
     size_t ldw;
-    int nsplit;
+    int nsplit;            // splits of a row at most
+    uint32_t split_least;  // keys of a split at least
     // workspace
     uint4* seen;     // [n_seqs]
     float2* part_ml; // [n_seqs][n_heads][nsplit]
@@ -731,7 +732,11 @@ struct PagedAttend {
     float* scores;   // [n_seqs][n_heads][score_ld] with weights
     size_t score_ld;
 };
-int paged_pick_splits(size_t n_seqs, size_t kv_heads, int group, uint32_t max_seen, int cu_count);
+struct PagedSplits {
+    int count;
+    uint32_t least;
+};
+PagedSplits paged_pick_splits(size_t n_seqs, size_t kv_heads, int group, uint32_t max_seen, bool window, int cu_count);
 hipError_t launch_paged_attend(hipStream_t s, const focr_hip_paged* c, const PagedAttend& a, focr_hip_ctx* ctx);
 hipError_t launch_paged_write(hipStream_t s, const focr_hip_paged* c, const float* k, const float* v, size_t ld,
                               size_t rows, const uint32_t* seq, const uint32_t* pos, const uint32_t* tables,

@@ -157,7 +157,10 @@ int32_t attend(focr_hip_ctx* ctx, const char* who, const focr_hip_paged* c, cons
     a.weights = weights;
     a.ldw = ldw;
     const size_t seen = window && !prefix ? std::min(max_len, window) : max_len;
-    a.nsplit = paged_pick_splits(n_seqs, c->n_kv_heads, a.group, static_cast<uint32_t>(seen), ctx->cu_count);
+    const PagedSplits splits = paged_pick_splits(n_seqs, c->n_kv_heads, a.group, static_cast<uint32_t>(seen), window != 0,
+                                                 ctx->cu_count);
+    a.nsplit = splits.count;
+    a.split_least = splits.least;
     if (check) {
         Check k{ctx};
         if ((st = k.begin(who))) return st;

@@ -13,6 +13,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "focr_internal.hpp"
 #include "k_common.hpp"
@@ -129,6 +130,27 @@ __device__ __forceinline__ float fold_lanes(float v, Op op) {
     return v;
 }
 
+// The rows of a split's keys b0 .. b0 + cnt, to LDS, with none behind them up
+// to `padded`. Every table entry of a thread is requested before the first is
+// used (one after the other they were eight waits of a loaded memory).
+__device__ __forceinline__ void fill_rows(const PagedTables& t, const PoolGeom& g, const Seen& e, int s, uint32_t hk,
+                                          uint32_t b0, int cnt, int padded, uint32_t* s_row) {
+    constexpr int N = kPagedChunkMax / 256;
+    uint32_t row[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (i * 256 < cnt) {  // uniform; past the end a thread takes the last key's again
+            const uint32_t at = b0 + min(static_cast<int>(threadIdx.x) + i * 256, cnt - 1);
+            row[i] = row_of(t, g, s, hk, at < e.p ? at : at + e.shift);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int j = static_cast<int>(threadIdx.x) + i * 256;
+        if (j < padded) s_row[j] = j < cnt ? row[i] : kBadRow;
+    }
+}
+
 // The four waves' maxima, sums and outputs of GT heads joined and written as
 // split z's part; row0: the first head's row of all [sequence][head].
 template <int GT, int D>
@@ -150,15 +172,15 @@ __device__ __forceinline__ void join_waves(const PagedAttend& a, const float (*s
     }
 }
 
-// One split of one key head's keys, for GT of its query heads. Grid (split,
-// key head x head tile, sequence), 4 waves. Every wave takes tiles of its own:
+// One split of one key head's keys, for its GT query heads (the group). Grid
+// (split, key head, sequence), 4 waves. Every wave takes tiles of its own:
 // C lanes hold a key's row (16 bytes each), 64 / C keys to a load
 // instruction, U of those for K and U for V in flight at once; a lane keeps
 // the same key's K and V, so the probabilities never leave their lanes, and
 // there is no barrier until the four waves' maxima, sums and outputs are
 // joined at the end.
 template <typename T, int D, int GT, int U>
-__global__ __launch_bounds__(256) void paged_attend_kernel(PoolGeom g, PagedAttend a) {
+__global__ __launch_bounds__(256, GT == 1 ? 4 : 3) void paged_attend_kernel(PoolGeom g, PagedAttend a) {
     constexpr int E = Row16<T>::N;
     constexpr int C = D / E;
     constexpr int R = 64 / C;
@@ -168,23 +190,18 @@ __global__ __launch_bounds__(256) void paged_attend_kernel(PoolGeom g, PagedAtte
     __shared__ float s_acc[4][GT][D];
     __shared__ float2 s_ml[4][GT];
     const int z = blockIdx.x;
-    const int tiles = (a.group + GT - 1) / GT;
-    const int hk = blockIdx.y / tiles;
-    const int g0 = (blockIdx.y - hk * tiles) * GT;  // the first of this block's query heads in the group
+    const int hk = blockIdx.y;
     const int s = blockIdx.z;
     const Seen e = seen_of(a.t, a.prefix, a.window, a.k_steps != nullptr, s);
     if (z == 0 && blockIdx.y == 0 && threadIdx.x == 0)
         a.seen[s] = make_uint4(e.none ? kPagedNone : e.nvis, e.p, e.shift, e.own ? 1u : 0u);
     if (e.none) return;
-    const uint32_t chunk = split_keys(e.nvis, a.nsplit);
+    const uint32_t chunk = split_keys(e.nvis, a.nsplit, a.split_least);
     const uint32_t b0 = static_cast<uint32_t>(z) * chunk;
     if (b0 >= e.nvis) return;
     const int cnt = static_cast<int>(min(chunk, e.nvis - b0));
     const int padded = (cnt + TILE - 1) / TILE * TILE;
-    for (int j = threadIdx.x; j < padded; j += 256) {
-        const uint32_t at = b0 + j;
-        s_row[j] = j < cnt ? row_of(a.t, g, s, hk, at < e.p ? at : at + e.shift) : kBadRow;
-    }
+    fill_rows(a.t, g, e, s, hk, b0, cnt, padded, s_row);
     const int wave = threadIdx.x >> 6;
     const int lane = threadIdx.x & 63;
     const int cl = lane % C;  // which 16 bytes of a row
@@ -193,9 +210,9 @@ __global__ __launch_bounds__(256) void paged_attend_kernel(PoolGeom g, PagedAtte
     const float qscale = a.scale * kLog2e;
 #pragma unroll
     for (int i = 0; i < GT; ++i) {
-        const float* qr = a.q + static_cast<size_t>(s) * a.ldq + (static_cast<size_t>(hk) * a.group + g0 + i) * D + cl * E;
+        const float* qr = a.q + static_cast<size_t>(s) * a.ldq + (static_cast<size_t>(hk) * GT + i) * D + cl * E;
 #pragma unroll
-        for (int j = 0; j < E; ++j) q[i][j] = g0 + i < a.group ? qr[j] * qscale : 0.0f;
+        for (int j = 0; j < E; ++j) q[i][j] = qr[j] * qscale;
     }
     // the step's own row is the last key seen
     const int own = e.own && e.nvis - 1 - b0 < static_cast<uint32_t>(cnt) ? static_cast<int>(e.nvis - 1 - b0) : -1;
@@ -210,8 +227,8 @@ __global__ __launch_bounds__(256) void paged_attend_kernel(PoolGeom g, PagedAtte
     __syncthreads();
     const u4* kp = static_cast<const u4*>(g.k) + cl;
     const u4* vp = static_cast<const u4*>(g.v) + cl;
-    const size_t head0 = static_cast<size_t>(hk) * a.group + g0;
-    const size_t n_heads = static_cast<size_t>(g.kv_heads) * a.group;
+    const size_t head0 = static_cast<size_t>(hk) * GT;
+    const size_t n_heads = static_cast<size_t>(g.kv_heads) * GT;
     for (int t0 = wave * TILE; t0 < cnt; t0 += 4 * TILE) {
         uint32_t row[U];
         bool all = true;
@@ -244,10 +261,8 @@ __global__ __launch_bounds__(256) void paged_attend_kernel(PoolGeom g, PagedAtte
 #pragma unroll
                     for (int j = 0; j < E; ++j) f[j] = a.v_steps[at + j];
                     vw[u] = Row16<T>::pack(f);
-                    if (g0 == 0) {
-                        static_cast<u4*>(g.k)[static_cast<size_t>(row[u]) * C + cl] = kw[u];
-                        static_cast<u4*>(g.v)[static_cast<size_t>(row[u]) * C + cl] = vw[u];
-                    }
+                    static_cast<u4*>(g.k)[static_cast<size_t>(row[u]) * C + cl] = kw[u];
+                    static_cast<u4*>(g.v)[static_cast<size_t>(row[u]) * C + cl] = vw[u];
                 }
             }
         }
@@ -272,8 +287,7 @@ __global__ __launch_bounds__(256) void paged_attend_kernel(PoolGeom g, PagedAtte
                 if (cl == 0 && j < cnt)
 #pragma unroll
                     for (int i = 0; i < GT; ++i)
-                        if (g0 + i < a.group)
-                            a.scores[(static_cast<size_t>(s) * n_heads + head0 + i) * a.score_ld + b0 + j] = sc[u][i];
+                        a.scores[(static_cast<size_t>(s) * n_heads + head0 + i) * a.score_ld + b0 + j] = sc[u][i];
             }
         }
         float safe[GT];
@@ -315,32 +329,99 @@ __global__ __launch_bounds__(256) void paged_attend_kernel(PoolGeom g, PagedAtte
             for (int j = 0; j < E; ++j) s_acc[wave][i][cl * E + j] = acc[i][j];
     }
     __syncthreads();
-    join_waves<GT, D>(a, s_acc, s_ml, g0, head0 + static_cast<size_t>(s) * n_heads, z);
+    join_waves<GT, D>(a, s_acc, s_ml, 0, head0 + static_cast<size_t>(s) * n_heads, z);
 }
 
-// The same split on the f32 matrix cores, for up to 16 query heads of a key
-// head at once (grid (split, key head x tile of 16 heads, sequence)). A wave
-// takes 16 keys at a time on v_mfma_f32_16x16x4_f32, lane l = 16 a + b:
-//   scores  S[key][head]: A = K (lane: key b, one of the row's 16-byte pieces
+// The same split on the matrix cores, for up to 16 query heads of a key head at
+// once (grid (split, key head x tile of 16 heads, sequence)). A wave takes 16
+// keys at a time; lane l = 16 a + b:
+//   scores  S[key][head] = K q: A = K (lane: key b, the row's 16-byte pieces
 //           a + 4 c), B = q (lane: head b, the same values of d). The result
 //           leaves lane l with head b and the keys 4 a + i, i < 4 ...
-//   output  O[head][d]: ... which is what A of step i takes (head b, key
-//           4 a + i), so the probabilities stay where they are; B = V (lane:
-//           key 4 a + i, pieces b + 16 c of its row, one value at a time).
-// The running maximum is moved only where a score is more than 2^8 times past
-// it (any reference gives the same quotient, and f32 holds the sums), so the
-// usual tile needs nothing from other lanes.
+//   output  O[head][d] = P V: ... which is what A takes here, so the
+//           probabilities stay where they are; B = V (lane: keys 4 a + i, one
+//           of the columns (b + 16 c) VE + j at a time).
+// An f32 cache runs v_mfma_f32_16x16x4_f32. A 16-bit cache's K and V are exact
+// operands of the 16-bit instructions (16x16x32 for the scores, 16x16x16 for
+// the output, at eight and four times the f32 rate); q and P are f32 and are
+// written as sums of 16-bit terms that hold their 24 bits: three of bf16, cut
+// off (exact), or two of f16, rounded (to 2^-23), after q's row is scaled by a
+// power of two to below 2^15 and P by 2^14, so that f16's exponents reach.
+// The terms do not hold infinities (an infinite K times a term that is zero is
+// NaN): a wave whose sums come out not finite does its keys again in f32.
+// The running maximum is moved only where a score is well past it (any
+// reference gives the same quotient, and f32 holds the sums), so the usual
+// tile needs nothing from other lanes.
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+
+template <typename T>
+struct Terms {  // f32: its own products alone
+    static constexpr bool kSplit = false;
+    static constexpr int N = 1;
+    static constexpr float kTop = 0.0f, kPast = 8.0f;
+    static __device__ void split2(float, float, uint32_t*) {}
+    static __device__ v4f scores(const u4&, const u4&, v4f c) { return c; }
+    static __device__ v4f output(const u2&, const u2&, v4f c) { return c; }
+};
+template <>
+struct Terms<__bf16> {
+    static constexpr bool kSplit = true;
+    static constexpr int N = 3;
+    static constexpr float kTop = 0.0f;   // the maximum's exponential is 2^kTop
+    static constexpr float kPast = 8.0f;  // how far a score may pass the reference
+    // two values' terms in one word each
+    static __device__ __forceinline__ void split2(float x, float y, uint32_t* w) {
+#pragma unroll
+        for (int t = 0; t < N; ++t) {
+            const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+            w[t] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+            x -= __uint_as_float(a & 0xFFFF0000u);
+            y -= __uint_as_float(b & 0xFFFF0000u);
+        }
+    }
+    static __device__ __forceinline__ v4f scores(const u4& k, const u4& q, v4f c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, k), __builtin_bit_cast(v8bf, q), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ v4f output(const u2& p, const u2& v, v4f c) {
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(v4s, p), __builtin_bit_cast(v4s, v), c, 0, 0, 0);
+    }
+};
+template <>
+struct Terms<_Float16> {
+    static constexpr bool kSplit = true;
+    static constexpr int N = 2;
+    static constexpr float kTop = 14.0f;
+    static constexpr float kPast = 15.0f;
+    static __device__ __forceinline__ void split2(float x, float y, uint32_t* w) {
+#pragma unroll
+        for (int t = 0; t < N; ++t) {
+            const _Float16 a = static_cast<_Float16>(x), b = static_cast<_Float16>(y);
+            w[t] = __builtin_bit_cast(uint16_t, a) | static_cast<uint32_t>(__builtin_bit_cast(uint16_t, b)) << 16;
+            x -= static_cast<float>(a);
+            y -= static_cast<float>(b);
+        }
+    }
+    static __device__ __forceinline__ v4f scores(const u4& k, const u4& q, v4f c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, k), __builtin_bit_cast(v8h, q), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ v4f output(const u2& p, const u2& v, v4f c) {
+        return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(v4h, p), __builtin_bit_cast(v4h, v), c, 0, 0, 0);
+    }
+};
 
 template <typename T, int D>
-__global__ __launch_bounds__(256) void paged_attend_mfma_kernel(PoolGeom g, PagedAttend a) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_attend_mfma_kernel(PoolGeom g, PagedAttend a) {
+    using TT = Terms<T>;
     constexpr int E = Row16<T>::N;
-    constexpr int C = D / E;                   // 16-byte pieces of a row
-    constexpr int KC = C / 4;                  // K pieces of a lane
-    constexpr int VE = C >= 16 ? E : E / 2;    // values of a V piece (8 bytes where a row has 8 pieces of 16)
-    constexpr int VC = D / (16 * VE);          // V pieces of a lane and key
-    constexpr int VD = VC * VE;                // output columns of a lane
+    constexpr int C = D / E;                 // 16-byte pieces of a row
+    constexpr int KC = C / 4;                // K pieces of a lane
+    constexpr int VE = C >= 16 ? E : E / 2;  // values of a V piece (8 bytes where a row has 8 pieces of 16)
+    constexpr int VC = D / (16 * VE);        // V pieces of a lane and key
     __shared__ uint32_t s_row[kPagedChunkMax];
     __shared__ float s_acc[4][16][D];
     __shared__ float2 s_ml[4][16];
@@ -353,15 +434,12 @@ __global__ __launch_bounds__(256) void paged_attend_mfma_kernel(PoolGeom g, Page
     if (z == 0 && blockIdx.y == 0 && threadIdx.x == 0)
         a.seen[s] = make_uint4(e.none ? kPagedNone : e.nvis, e.p, e.shift, e.own ? 1u : 0u);
     if (e.none) return;
-    const uint32_t chunk = split_keys(e.nvis, a.nsplit);
+    const uint32_t chunk = split_keys(e.nvis, a.nsplit, a.split_least);
     const uint32_t b0 = static_cast<uint32_t>(z) * chunk;
     if (b0 >= e.nvis) return;
     const int cnt = static_cast<int>(min(chunk, e.nvis - b0));
     const int padded = (cnt + 15) & ~15;
-    for (int j = threadIdx.x; j < padded; j += 256) {
-        const uint32_t at = b0 + j;
-        s_row[j] = j < cnt ? row_of(a.t, g, s, hk, at < e.p ? at : at + e.shift) : kBadRow;
-    }
+    fill_rows(a.t, g, e, s, hk, b0, cnt, padded, s_row);
     const int wave = threadIdx.x >> 6;
     const int lane = threadIdx.x & 63;
     const int la = lane >> 4;
@@ -369,27 +447,12 @@ __global__ __launch_bounds__(256) void paged_attend_mfma_kernel(PoolGeom g, Page
     const bool head = g0 + lb < a.group;
     const size_t head0 = static_cast<size_t>(hk) * a.group + g0;
     const size_t n_heads = static_cast<size_t>(g.kv_heads) * a.group;
-    float q[KC][E];
-    {
-        const float* qr = a.q + static_cast<size_t>(s) * a.ldq + (head0 + lb) * D + la * E;
-        const float qscale = a.scale * kLog2e;
-#pragma unroll
-        for (int c = 0; c < KC; ++c)
-#pragma unroll
-            for (int j = 0; j < E; ++j) q[c][j] = head ? qr[4 * E * c + j] * qscale : 0.0f;
-    }
+    // a lane without a head reads the last one's row and takes zeros
+    const float* qr = a.q + static_cast<size_t>(s) * a.ldq + (static_cast<size_t>(hk) * a.group + min(g0 + lb, a.group - 1)) * D + la * E;
+    const float qscale = a.scale * kLog2e;
     const int own = e.own && e.nvis - 1 - b0 < static_cast<uint32_t>(cnt) ? static_cast<int>(e.nvis - 1 - b0) : -1;
-    float m = -INFINITY, l = 0.0f;  // of head lb, this lane's keys
-    v4f acc[VC][VE];                // of heads 4 la + r, columns (lb + 16 c) VE + j
-#pragma unroll
-    for (int c = 0; c < VC; ++c)
-#pragma unroll
-        for (int j = 0; j < VE; ++j) acc[c][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    __syncthreads();
-    struct Tile {
-        uint32_t krow, vrow[4];
-        u4 kw[KC], vw[4][VC];
-    };
+    float m, l;         // of head lb, this lane's keys
+    v4f acc[VC][VE];    // of heads 4 la + r, columns (lb + 16 c) VE + j
     const u4* kp = static_cast<const u4*>(g.k) + la;
     const auto vload = [&](uint32_t row, int c) -> u4 {
         const char* p = static_cast<const char*>(g.v) + (static_cast<size_t>(row) * D + (lb + 16 * c) * VE) * sizeof(T);
@@ -400,115 +463,192 @@ __global__ __launch_bounds__(256) void paged_attend_mfma_kernel(PoolGeom g, Page
             return *reinterpret_cast<const u4*>(p);
         }
     };
-    const auto fetch = [&](Tile& t, int t0) {
-        t.krow = s_row[t0 + lb];
-        const uint4 vrow4 = *reinterpret_cast<const uint4*>(s_row + t0 + 4 * la);
-        t.vrow[0] = vrow4.x;
-        t.vrow[1] = vrow4.y;
-        t.vrow[2] = vrow4.z;
-        t.vrow[3] = vrow4.w;
-        if (__all(t.krow != kBadRow)) {
+    const auto run = [&](auto f32_products) {
+        constexpr bool EXACT = decltype(f32_products)::value;
+        m = -INFINITY;
+        l = 0.0f;
 #pragma unroll
-            for (int c = 0; c < KC; ++c) t.kw[c] = kp[static_cast<size_t>(t.krow) * C + 4 * c];
+        for (int c = 0; c < VC; ++c)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int j = 0; j < VE; ++j) acc[c][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        float q[KC][E];
 #pragma unroll
-                for (int c = 0; c < VC; ++c) t.vw[i][c] = vload(t.vrow[i], c);
-        } else {  // slots that hold no key are not read: what lies there may be NaN
+        for (int c = 0; c < KC; ++c)
 #pragma unroll
-            for (int c = 0; c < KC; ++c)
-                t.kw[c] = t.krow != kBadRow ? kp[static_cast<size_t>(t.krow) * C + 4 * c] : u4{0, 0, 0, 0};
+            for (int j = 0; j < E; ++j) q[c][j] = qr[4 * E * c + j] * qscale;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+        for (int c = 0; c < KC; ++c)
 #pragma unroll
-                for (int c = 0; c < VC; ++c) t.vw[i][c] = t.vrow[i] != kBadRow ? vload(t.vrow[i], c) : u4{0, 0, 0, 0};
-        }
-    };
-    const auto attend = [&](Tile& t, int t0) {
-        uint32_t (&vrow)[4] = t.vrow;
-        const uint32_t krow = t.krow;
-        u4 (&kw)[KC] = t.kw;
-        u4 (&vw)[4][VC] = t.vw;
-        if (own >= t0 && own < t0 + 16) {  // the step's row comes from the call and goes to its page
-            const size_t at = static_cast<size_t>(s) * a.ldkv + static_cast<size_t>(hk) * D;
-            float f[8];
-            if (t0 + lb == own && krow != kBadRow) {
+            for (int j = 0; j < E; ++j) q[c][j] = head ? q[c][j] : 0.0f;
+        u4 qt[TT::N][KC];
+        float unscale = 1.0f;
+        if constexpr (!EXACT) {
+            if constexpr (TT::kTop != 0.0f) {  // a power of two that brings the row below 2^15
+                float big = 0.0f;
 #pragma unroll
-                for (int c = 0; c < KC; ++c) {
+                for (int c = 0; c < KC; ++c)
 #pragma unroll
-                    for (int j = 0; j < E; ++j) f[j] = a.k_steps[at + (la + 4 * c) * E + j];
-                    kw[c] = Row16<T>::pack(f);
-                    if (g0 == 0) static_cast<u4*>(g.k)[static_cast<size_t>(krow) * C + la + 4 * c] = kw[c];
-                }
+                    for (int j = 0; j < E; ++j) big = fmaxf(big, fabsf(q[c][j]));
+                big = fold_lanes<16, 64>(big, Max());
+                const int up = big > 0.0f && big < INFINITY ? min(max(14 - ilogbf(big), -100), 100) : 0;
+                unscale = ldexpf(1.0f, -up);
+                const float by = ldexpf(1.0f, up);
+#pragma unroll
+                for (int c = 0; c < KC; ++c)
+#pragma unroll
+                    for (int j = 0; j < E; ++j) q[c][j] *= by;
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (t0 + 4 * la + i == own && vrow[i] != kBadRow) {
+            for (int c = 0; c < KC; ++c)
 #pragma unroll
-                    for (int c = 0; c < VC; ++c) {
+                for (int j = 0; j < E; j += 2) {
+                    uint32_t w[TT::N];
+                    TT::split2(q[c][j], q[c][j + 1], w);
 #pragma unroll
-                        for (int j = 0; j < E; ++j) f[j] = j < VE ? a.v_steps[at + (lb + 16 * c) * VE + j] : 0.0f;
-                        vw[i][c] = Row16<T>::pack(f);
-                        if (g0 == 0) {
-                            char* p = static_cast<char*>(g.v) + (static_cast<size_t>(vrow[i]) * D + (lb + 16 * c) * VE) * sizeof(T);
-                            if constexpr (VE * sizeof(T) == 8)
-                                *reinterpret_cast<u2*>(p) = u2{vw[i][c][0], vw[i][c][1]};
-                            else
-                                *reinterpret_cast<u4*>(p) = vw[i][c];
+                    for (int t = 0; t < TT::N; ++t) qt[t][c][j / 2] = w[t];
+                }
+        }
+        for (int t0 = wave * 16; t0 < cnt; t0 += 64) {
+            const uint32_t krow = s_row[t0 + lb];
+            const uint4 vrow4 = *reinterpret_cast<const uint4*>(s_row + t0 + 4 * la);
+            const uint32_t vrow[4] = {vrow4.x, vrow4.y, vrow4.z, vrow4.w};
+            u4 kw[KC], vw[4][VC];
+            if (__all(krow != kBadRow)) {
+#pragma unroll
+                for (int c = 0; c < KC; ++c) kw[c] = kp[static_cast<size_t>(krow) * C + 4 * c];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int c = 0; c < VC; ++c) vw[i][c] = vload(vrow[i], c);
+            } else {  // slots that hold no key are not read: what lies there may be NaN
+#pragma unroll
+                for (int c = 0; c < KC; ++c) kw[c] = krow != kBadRow ? kp[static_cast<size_t>(krow) * C + 4 * c] : u4{0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int c = 0; c < VC; ++c) vw[i][c] = vrow[i] != kBadRow ? vload(vrow[i], c) : u4{0, 0, 0, 0};
+            }
+            if (own >= t0 && own < t0 + 16) {  // the step's row comes from the call and goes to its page
+                const size_t at = static_cast<size_t>(s) * a.ldkv + static_cast<size_t>(hk) * D;
+                float f[8];
+                if (t0 + lb == own && krow != kBadRow) {
+#pragma unroll
+                    for (int c = 0; c < KC; ++c) {
+#pragma unroll
+                        for (int j = 0; j < E; ++j) f[j] = a.k_steps[at + (la + 4 * c) * E + j];
+                        kw[c] = Row16<T>::pack(f);
+                        if (g0 == 0) static_cast<u4*>(g.k)[static_cast<size_t>(krow) * C + la + 4 * c] = kw[c];
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (t0 + 4 * la + i == own && vrow[i] != kBadRow) {
+#pragma unroll
+                        for (int c = 0; c < VC; ++c) {
+#pragma unroll
+                            for (int j = 0; j < E; ++j) f[j] = j < VE ? a.v_steps[at + (lb + 16 * c) * VE + j] : 0.0f;
+                            vw[i][c] = Row16<T>::pack(f);
+                            if (g0 == 0) {
+                                char* p = static_cast<char*>(g.v) + (static_cast<size_t>(vrow[i]) * D + (lb + 16 * c) * VE) * sizeof(T);
+                                if constexpr (VE * sizeof(T) == 8)
+                                    *reinterpret_cast<u2*>(p) = u2{vw[i][c][0], vw[i][c][1]};
+                                else
+                                    *reinterpret_cast<u4*>(p) = vw[i][c];
+                            }
                         }
                     }
                 }
             }
-        }
-        v4f sc = {0.0f, 0.0f, 0.0f, 0.0f};
+            v4f sc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int c = 0; c < KC; ++c) {
-            float f[E];
-            Row16<T>::load(kw[c], f);
+            for (int c = 0; c < KC; ++c) {
+                if constexpr (EXACT) {
+                    float f[E];
+                    Row16<T>::load(kw[c], f);
 #pragma unroll
-            for (int j = 0; j < E; ++j) sc = __builtin_amdgcn_mfma_f32_16x16x4f32(f[j], q[c][j], sc, 0, 0, 0);
-        }
+                    for (int j = 0; j < E; ++j) sc = __builtin_amdgcn_mfma_f32_16x16x4f32(f[j], q[c][j], sc, 0, 0, 0);
+                } else {  // the small terms first
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[i] = vrow[i] != kBadRow ? sc[i] : -INFINITY;
-        if (a.scores && head) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (t0 + 4 * la + i < cnt)
-                    a.scores[(static_cast<size_t>(s) * n_heads + head0 + lb) * a.score_ld + b0 + t0 + 4 * la + i] = sc[i];
-        }
-        float mx = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
-        if (__any(mx > m + 8.0f)) {
-            mx = fmaxf(fold_lanes<16, 64>(mx, Max()), m);
-            const float corr = __builtin_amdgcn_exp2f(m - (mx == -INFINITY ? 0.0f : mx));
-            m = mx;
-            l *= corr;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float cr = __shfl(corr, 4 * la + r, 64);
-#pragma unroll
-                for (int c = 0; c < VC; ++c)
-#pragma unroll
-                    for (int j = 0; j < VE; ++j) acc[c][j][r] *= cr;
+                    for (int t = TT::N - 1; t >= 0; --t) sc = TT::scores(kw[c], qt[t][c], sc);
+                }
             }
-        }
-        const float safe = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float p = __builtin_amdgcn_exp2f(sc[i] - safe);
-            l += p;
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (!EXACT && TT::kTop != 0.0f) sc[i] *= unscale;
+                sc[i] = vrow[i] != kBadRow ? sc[i] : -INFINITY;
+            }
+            if (a.scores && head) {
 #pragma unroll
-            for (int c = 0; c < VC; ++c) {
-                float f[E];
-                Row16<T>::load(vw[i][c], f);
+                for (int i = 0; i < 4; ++i)
+                    if (t0 + 4 * la + i < cnt)
+                        a.scores[(static_cast<size_t>(s) * n_heads + head0 + lb) * a.score_ld + b0 + t0 + 4 * la + i] = sc[i];
+            }
+            float mx = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
+            if (__any(mx > m + TT::kPast)) {
+                mx = fmaxf(fold_lanes<16, 64>(mx, Max()) - TT::kTop, m);
+                const float corr = __builtin_amdgcn_exp2f(m - (mx == -INFINITY ? 0.0f : mx));
+                m = mx;
+                l *= corr;
 #pragma unroll
-                for (int j = 0; j < VE; ++j) acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(p, f[j], acc[c][j], 0, 0, 0);
+                for (int r = 0; r < 4; ++r) {
+                    const float cr = __shfl(corr, 4 * la + r, 64);
+#pragma unroll
+                    for (int c = 0; c < VC; ++c)
+#pragma unroll
+                        for (int j = 0; j < VE; ++j) acc[c][j][r] *= cr;
+                }
+            }
+            const float safe = m == -INFINITY ? 0.0f : m;
+            float p[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                p[i] = __builtin_amdgcn_exp2f(sc[i] - safe);
+                l += p[i];
+            }
+            if constexpr (EXACT) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int c = 0; c < VC; ++c) {
+                        float f[E];
+                        Row16<T>::load(vw[i][c], f);
+#pragma unroll
+                        for (int j = 0; j < VE; ++j) acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[i], f[j], acc[c][j], 0, 0, 0);
+                    }
+            } else {
+                uint32_t w0[TT::N], w1[TT::N];
+                TT::split2(p[0], p[1], w0);
+                TT::split2(p[2], p[3], w1);
+#pragma unroll
+                for (int c = 0; c < VC; ++c) {
+                    u2 v[VE];
+#pragma unroll
+                    for (int j = 0; j < VE; ++j) {  // a column of the four keys: halves of their words
+                        const uint32_t sel = j & 1 ? 0x07060302u : 0x05040100u;
+                        v[j] = u2{__builtin_amdgcn_perm(vw[1][c][j / 2], vw[0][c][j / 2], sel),
+                                  __builtin_amdgcn_perm(vw[3][c][j / 2], vw[2][c][j / 2], sel)};
+                    }
+#pragma unroll
+                    for (int t = TT::N - 1; t >= 0; --t)  // independent products between those of one sum
+#pragma unroll
+                        for (int j = 0; j < VE; ++j) acc[c][j] = TT::output(u2{w0[t], w1[t]}, v[j], acc[c][j]);
+                }
             }
         }
     };
-    for (int t0 = wave * 16; t0 < cnt; t0 += 64) {
-        Tile t;
-        fetch(t, t0);
-        attend(t, t0);
+    __syncthreads();
+    if constexpr (!TT::kSplit) {
+        run(std::true_type{});
+    } else {
+        run(std::false_type{});
+        float bad = l * 0.0f;  // NaN where a sum is not finite
+#pragma unroll
+        for (int c = 0; c < VC; ++c)
+#pragma unroll
+            for (int j = 0; j < VE; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) bad += acc[c][j][r] * 0.0f;
+        if (__any(bad != bad)) run(std::true_type{});
     }
     l = fold_lanes<16, 64>(l, Sum());
     if (lane < 16) s_ml[wave][lane] = make_float2(m, l);
@@ -537,7 +677,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttend a) {
     const uint4 e = a.seen[s];
     if (e.x == kPagedNone) return;
     const uint32_t nvis = e.x;
-    const int n = static_cast<int>((nvis + split_keys(nvis, a.nsplit) - 1) / split_keys(nvis, a.nsplit));
+    const int n = static_cast<int>((nvis + split_keys(nvis, a.nsplit, a.split_least) - 1) / split_keys(nvis, a.nsplit, a.split_least));
     const size_t part = (static_cast<size_t>(s) * gridDim.x + h) * a.nsplit;
     float m = -INFINITY;
     for (int z = threadIdx.x; z < n; z += 256) m = fmaxf(m, a.part_ml[part + z].x);
@@ -588,7 +728,7 @@ __global__ __launch_bounds__(256) void paged_weights_kernel(PagedAttend a) {
     if (e.x == kPagedNone) return;
     const uint32_t nvis = e.x;
     if (blockIdx.x * 256u >= nvis) return;
-    const int n = static_cast<int>((nvis + split_keys(nvis, a.nsplit) - 1) / split_keys(nvis, a.nsplit));
+    const int n = static_cast<int>((nvis + split_keys(nvis, a.nsplit, a.split_least) - 1) / split_keys(nvis, a.nsplit, a.split_least));
     const size_t n_heads = static_cast<size_t>(gridDim.y) * a.group;
     const size_t head0 = static_cast<size_t>(s) * n_heads + static_cast<size_t>(hk) * a.group;
     for (int i = threadIdx.x >> 6; i < a.group; i += 4) {  // a wave a head
@@ -1038,14 +1178,12 @@ void attend(hipStream_t s, const focr_hip_paged* c, const PagedAttend& a) {
     const PoolGeom g = geom_of(c);
     const int kv = static_cast<int>(c->n_kv_heads);
     const auto grid = [&](int gt) { return dim3(a.nsplit, kv * ((a.group + gt - 1) / gt), a.t.n_seqs); };
-    if (a.group == 1)
-        FOCR_LAUNCH((paged_attend_kernel<T, D, 1, 8>), grid(1), dim3(256), 0, s, g, a);
+    if (a.group > 2)
+        FOCR_LAUNCH((paged_attend_mfma_kernel<T, D>), grid(16), dim3(256), 0, s, g, a);
     else if (a.group == 2)
         FOCR_LAUNCH((paged_attend_kernel<T, D, 2, 8>), grid(2), dim3(256), 0, s, g, a);
-    else if (a.group <= 4)
-        FOCR_LAUNCH((paged_attend_kernel<T, D, 4, 4>), grid(4), dim3(256), 0, s, g, a);
     else
-        FOCR_LAUNCH((paged_attend_mfma_kernel<T, D>), grid(16), dim3(256), 0, s, g, a);
+        FOCR_LAUNCH((paged_attend_kernel<T, D, 1, 8>), grid(1), dim3(256), 0, s, g, a);
 }
 
 template <typename T>
@@ -1060,8 +1198,8 @@ void attend_dim(hipStream_t s, const focr_hip_paged* c, const PagedAttend& a) {
 
 }  // namespace
 
-int paged_pick_splits(size_t n_seqs, size_t kv_heads, int group, uint32_t max_seen, int cu_count) {
-    return pick_splits(n_seqs, kv_heads, group, max_seen, cu_count);
+PagedSplits paged_pick_splits(size_t n_seqs, size_t kv_heads, int group, uint32_t max_seen, bool window, int cu_count) {
+    return pick_splits(n_seqs, kv_heads, group, max_seen, window, cu_count);
 }
 
 hipError_t launch_paged_attend(hipStream_t s, const focr_hip_paged* c, const PagedAttend& a, focr_hip_ctx* ctx) {

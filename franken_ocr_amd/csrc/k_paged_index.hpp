@@ -57,22 +57,26 @@ FOCR_INDEX Seen seen_of(const PagedTables& t, const uint32_t* prefix, uint32_t w
     return e;
 }
 
-// Keys of one split: the visible ones over at most nsplit splits, in whole units.
-FOCR_INDEX uint32_t split_keys(uint32_t nvis, int nsplit) {
+// Keys of one split: at least `least`, and enough for the visible ones to make
+// at most nsplit splits, in whole units.
+FOCR_INDEX uint32_t split_keys(uint32_t nvis, int nsplit, uint32_t least) {
     const uint32_t each = (nvis + nsplit - 1) / nsplit;
-    return umax32((each + kPagedChunkUnit - 1) / kPagedChunkUnit, 1u) * kPagedChunkUnit;
+    return umax32((each + kPagedChunkUnit - 1) / kPagedChunkUnit * kPagedChunkUnit, least);
 }
 
-// Splits of a call. Enough blocks for every CU to hold several, splits of at
-// most kPagedChunkMax keys (their rows are kept in LDS) and of at least
-// kPagedChunkUnit.
-inline int pick_splits(size_t n_seqs, size_t kv_heads, int group, uint32_t max_seen, int cu_count) {
-    const size_t tiles = static_cast<size_t>((group + 15) / 16);
-    const size_t base = std::max<size_t>(n_seqs * kv_heads * tiles, 1);
-    const size_t least = (static_cast<size_t>(max_seen) + kPagedChunkMax - 1) / kPagedChunkMax;
-    const size_t most = (static_cast<size_t>(max_seen) + kPagedChunkUnit - 1) / kPagedChunkUnit;
-    const size_t fill = (6 * static_cast<size_t>(cu_count) + base - 1) / base;
-    return static_cast<int>(std::max<size_t>(std::min(std::max(fill, least), most), 1));
+// Splits of a call whose sequences see up to max_seen keys: as many as give
+// every CU twelve blocks were all that long, of at most kPagedChunkMax keys (their
+// rows are kept in LDS). Sequences that are shorter get fewer splits of the
+// same length, so that blocks are alike (ragged lengths: equal counts of
+// unequal splits left CUs idle a quarter of the time); but where a window hides
+// most of what max_seen counts, what is seen is divided by the count.
+inline PagedSplits pick_splits(size_t n_seqs, size_t kv_heads, int group, uint32_t max_seen, bool window, int cu_count) {
+    const uint64_t rows = n_seqs * kv_heads * static_cast<uint64_t>((group + 15) / 16);
+    const uint64_t unit = kPagedChunkUnit;
+    const uint64_t even = (rows * max_seen + 12 * static_cast<uint64_t>(cu_count) - 1) / (12 * static_cast<uint64_t>(cu_count));
+    const uint64_t keys = std::min<uint64_t>(std::max<uint64_t>((even + unit - 1) / unit, 1) * unit, kPagedChunkMax);
+    const uint64_t count = std::max<uint64_t>((max_seen + keys - 1) / keys, 1);
+    return PagedSplits{static_cast<int>(count), static_cast<uint32_t>(window ? unit : keys)};
 }
 
 // The row (of head_dim elements) of key `key` of sequence s and head hk.

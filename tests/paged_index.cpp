@@ -42,9 +42,10 @@ int main() {
         require(e.own == (step && len < max_len), "own", at);
         const uint32_t seen = window && !with_prefix ? std::min(max_len, window) : max_len;
         require(e.nvis <= seen, "the call is sized for what is seen", at);
-        const int nsplit = pick_splits(n_seqs, heads, group, seen, 256);
+        const PagedSplits splits = pick_splits(n_seqs, heads, group, seen, window != 0, 256);
+        const int nsplit = splits.count;
         require(nsplit >= 1, "splits", at);
-        const uint32_t chunk = split_keys(e.nvis, nsplit);
+        const uint32_t chunk = split_keys(e.nvis, nsplit, splits.least);
         require(chunk <= static_cast<uint32_t>(kPagedChunkMax) && chunk % kPagedChunkUnit == 0, "a split fits LDS", at);
         std::vector<uint8_t> hit(max_pages << shift, 0);
         uint32_t covered = 0;
