@@ -392,7 +392,7 @@ __device__ __forceinline__ void permute_columns(const uint32_t* parent, int W, s
             if (b < W && parent[b] != static_cast<uint32_t>(b)) v[b] = *at(parent[b], i);
 #pragma unroll
         for (int b = 0; b < WB; ++b)
-            if (b < W && parent[b] != static_cast<uint32_t>(b)) *at(b, i) = v[b];
+            if (b < W && parent[b] != static_cast<uint32_t>(b)) __builtin_nontemporal_store(v[b], at(b, i));
     }
 }
 

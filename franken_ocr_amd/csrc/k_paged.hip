@@ -662,23 +662,20 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_attend_mfma_kerne
     join_waves<16, D>(a, s_acc, s_ml, g0, head0 + static_cast<size_t>(s) * n_heads, z);
 }
 
-// Grid (head, sequence): the splits of a row joined, out = sum_z acc_z f_z /
-// sum_z l_z f_z with f_z = exp2(m_z - max m), in the order of the splits
-// within each of the 256 / (D / 4) groups of lanes, then over the groups.
+// The splits of a row joined, out = sum_z acc_z f_z / sum_z l_z f_z with f_z =
+// exp2(m_z - max m), in the order of the splits within each of the 256 / (D /
+// 4) groups of lanes, then over the groups.
 template <int D>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttend a) {
+__device__ __forceinline__ void join_row(const PagedAttend& a, int h, int n_heads, int s, const uint4& e) {
     constexpr int L4 = D / 4;
     constexpr int G = 256 / L4;
     __shared__ float4 s_acc[G][L4];
     __shared__ float s_l[G];
     __shared__ float s_m[4];
-    const int h = blockIdx.x;
-    const int s = blockIdx.y;
-    const uint4 e = a.seen[s];
-    if (e.x == kPagedNone) return;
     const uint32_t nvis = e.x;
-    const int n = static_cast<int>((nvis + split_keys(nvis, a.nsplit, a.split_least) - 1) / split_keys(nvis, a.nsplit, a.split_least));
-    const size_t part = (static_cast<size_t>(s) * gridDim.x + h) * a.nsplit;
+    const uint32_t keys = split_keys(nvis, a.nsplit, a.split_least);
+    const int n = static_cast<int>((nvis + keys - 1) / keys);
+    const size_t part = (static_cast<size_t>(s) * n_heads + h) * a.nsplit;
     float m = -INFINITY;
     for (int z = threadIdx.x; z < n; z += 256) m = fmaxf(m, a.part_ml[part + z].x);
     m = wave_max_f_full(m);
@@ -718,19 +715,16 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttend a) {
     if (a.lens_advance && h == 0 && threadIdx.x == 0 && e.w != 0) a.lens_advance[s] += 1;
 }
 
-// Grid (256 keys, key head, sequence): weights[key] += sum over the head's
-// query heads of exp2(score - M) / L, M and L joined from the splits again.
-__global__ __launch_bounds__(256) void paged_weights_kernel(PagedAttend a) {
+// weights[key] += sum over the key head's query heads of exp2(score - M) / L
+// for kWeightKeys keys from j0 on, M and L joined from the splits again.
+constexpr int kWeightKeys = 512;
+__device__ __forceinline__ void add_weights(const PagedAttend& a, int hk, int kv_heads, int s, const uint4& e, uint32_t j0) {
     __shared__ float2 s_ml[64];
-    const int hk = blockIdx.y;
-    const int s = blockIdx.z;
-    const uint4 e = a.seen[s];
-    if (e.x == kPagedNone) return;
     const uint32_t nvis = e.x;
-    if (blockIdx.x * 256u >= nvis) return;
-    const int n = static_cast<int>((nvis + split_keys(nvis, a.nsplit, a.split_least) - 1) / split_keys(nvis, a.nsplit, a.split_least));
-    const size_t n_heads = static_cast<size_t>(gridDim.y) * a.group;
-    const size_t head0 = static_cast<size_t>(s) * n_heads + static_cast<size_t>(hk) * a.group;
+    if (j0 >= nvis) return;
+    const uint32_t keys = split_keys(nvis, a.nsplit, a.split_least);
+    const int n = static_cast<int>((nvis + keys - 1) / keys);
+    const size_t head0 = (static_cast<size_t>(s) * kv_heads + hk) * a.group;
     for (int i = threadIdx.x >> 6; i < a.group; i += 4) {  // a wave a head
         const float2* ml = a.part_ml + (head0 + i) * a.nsplit;
         float m = -INFINITY, l = 0.0f;
@@ -742,15 +736,30 @@ __global__ __launch_bounds__(256) void paged_weights_kernel(PagedAttend a) {
         if ((threadIdx.x & 63) == 0) s_ml[i] = make_float2(sf, l);
     }
     __syncthreads();
-    const uint32_t j = blockIdx.x * 256u + threadIdx.x;
-    if (j >= nvis) return;
-    float w = 0.0f;
-    for (int i = 0; i < a.group; ++i) {
-        const float sc = a.scores[(head0 + i) * a.score_ld + j];
-        w += __builtin_amdgcn_exp2f(sc - s_ml[i].x) / s_ml[i].y;
+    const uint32_t end = min(j0 + kWeightKeys, nvis);
+    for (uint32_t j = j0 + threadIdx.x; j < end; j += 256) {
+        float w = 0.0f;
+        for (int i = 0; i < a.group; ++i)
+            w += __builtin_amdgcn_exp2f(a.scores[(head0 + i) * a.score_ld + j] - s_ml[i].x) / s_ml[i].y;
+        const uint32_t key = j < e.y ? j : j + e.z;
+        a.weights[(static_cast<size_t>(s) * kv_heads + hk) * a.ldw + key] += w;
     }
-    const uint32_t key = j < e.y ? j : j + e.z;
-    a.weights[(static_cast<size_t>(s) * gridDim.y + hk) * a.ldw + key] += w;
+}
+
+// Grid (head, then chunk of keys x key head where weights are gathered;
+// sequence). The lengths are read from what the splits' launch noted: a step
+// counts them up here.
+template <int D>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttend a, int kv_heads) {
+    const int s = blockIdx.y;
+    const uint4 e = a.seen[s];
+    if (e.x == kPagedNone) return;
+    const int n_heads = kv_heads * a.group;
+    const int b = static_cast<int>(blockIdx.x) - n_heads;
+    if (b < 0)
+        join_row<D>(a, blockIdx.x, n_heads, s, e);
+    else
+        add_weights(a, b % kv_heads, kv_heads, s, e, static_cast<uint32_t>(b / kv_heads) * kWeightKeys);
 }
 
 // Rows of k / v [rows][kv_heads * D] into the slots (seq, pos) of the cache;
@@ -806,17 +815,25 @@ struct Pick {
     uint32_t found, want;  // the digits so far; how many of the keys that share them stay
 };
 
+// The sum of this lane's and the lower lanes' values: shifts within the 16-lane
+// rows, then row 0's and 2's last lanes to the rows behind them, then lane 31's.
+__device__ __forceinline__ uint32_t wave_prefix(uint32_t v) {
+    int x = static_cast<int>(v);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);  // row_shr:1
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
+    return static_cast<uint32_t>(x);
+}
+
 // Bins from the top until `want` keys are counted; hist in LDS or registers:
 // thread t holds the counts of bins 2047 - 2 t and 2046 - 2 t.
 __device__ __forceinline__ Pick find_digit(uint32_t hi, uint32_t lo, Pick p, int shift, uint32_t* s_wave, Pick* s_pick) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const uint32_t sum = hi + lo;
-    uint32_t incl = sum;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t v = __shfl_up(incl, o, 64);
-        incl += lane >= o ? v : 0u;
-    }
+    const uint32_t incl = wave_prefix(sum);
     if (lane == 63) s_wave[wave] = incl;
     __syncthreads();
     uint32_t before = incl - sum;
@@ -1054,13 +1071,17 @@ __global__ __launch_bounds__(kSelThreads) void paged_place_kernel(PagedEvict a, 
     t.place(c, p, above, equal, s_n, a.kept + row * a.budget, a.dst_weights + row * a.dst_ldw);
 }
 
+// Rows of a thread: 8 x 8192 -> 2048 slots took 52 us at 1, 53 at 2, 58 at 4 and
+// 87 at 8; stores past the caches made that 46 at 2 (52 at 4).
+constexpr int kGatherRows = 2;
+
 // Grid (tile of kept slots, key head, sequence): their rows into the pages of
 // dst_tables, 16 bytes a lane. The new lengths are written here: dst_lens may
 // be lens, and min(length, budget) is the same of the old and the new.
 template <int C>
 __global__ __launch_bounds__(256) void paged_gather_kernel(PoolGeom g, PagedEvict a) {
     constexpr int R = 256 / C;  // rows a step
-    constexpr int U = 4;
+    constexpr int U = kGatherRows;
     const int hk = blockIdx.y;
     const int s = blockIdx.z;
     const uint32_t len = a.t.lens[s];
@@ -1095,8 +1116,8 @@ __global__ __launch_bounds__(256) void paged_gather_kernel(PoolGeom g, PagedEvic
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         if (to[u] != kBadRow) {
-            static_cast<u4*>(g.k)[static_cast<size_t>(to[u]) * C + cl] = kw[u];
-            static_cast<u4*>(g.v)[static_cast<size_t>(to[u]) * C + cl] = vw[u];
+            __builtin_nontemporal_store(kw[u], static_cast<u4*>(g.k) + static_cast<size_t>(to[u]) * C + cl);
+            __builtin_nontemporal_store(vw[u], static_cast<u4*>(g.v) + static_cast<size_t>(to[u]) * C + cl);
         }
     }
 }
@@ -1215,19 +1236,15 @@ hipError_t launch_paged_attend(hipStream_t s, const focr_hip_paged* c, const Pag
     }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    if (a.weights) {
-        ProfScope ps(ctx, "paged_weights");
-        FOCR_LAUNCH(paged_weights_kernel, dim3((a.t.max_len + 255) / 256, kv, a.t.n_seqs), dim3(256), 0, s, a);
-        if ((e = hipGetLastError()) != hipSuccess) return e;
-    }
     ProfScope ps(ctx, "paged_join");
-    const dim3 grid(kv * a.group, a.t.n_seqs);
+    const uint32_t chunks = a.weights ? (a.t.max_len + kWeightKeys - 1) / kWeightKeys : 0;
+    const dim3 grid(kv * (a.group + chunks), a.t.n_seqs);
     if (c->head_dim == 64)
-        FOCR_LAUNCH(paged_join_kernel<64>, grid, dim3(256), 0, s, a);
+        FOCR_LAUNCH(paged_join_kernel<64>, grid, dim3(256), 0, s, a, kv);
     else if (c->head_dim == 128)
-        FOCR_LAUNCH(paged_join_kernel<128>, grid, dim3(256), 0, s, a);
+        FOCR_LAUNCH(paged_join_kernel<128>, grid, dim3(256), 0, s, a, kv);
     else
-        FOCR_LAUNCH(paged_join_kernel<256>, grid, dim3(256), 0, s, a);
+        FOCR_LAUNCH(paged_join_kernel<256>, grid, dim3(256), 0, s, a, kv);
     return hipGetLastError();
 }
 
@@ -1279,7 +1296,7 @@ hipError_t launch_paged_evict(hipStream_t s, const focr_hip_paged* c, const Page
     ProfScope ps(ctx, "paged_gather");
     const uint32_t most = std::min(a.budget, a.t.max_len);
     const int lanes = static_cast<int>(c->head_dim * c->esize() / 16);
-    const uint32_t rows = 4 * (256 / lanes);
+    const uint32_t rows = kGatherRows * (256 / lanes);
     const dim3 grid(std::max<uint32_t>((most + rows - 1) / rows, 1), g.kv_heads, a.t.n_seqs);
     if (lanes == 8)
         FOCR_LAUNCH(paged_gather_kernel<8>, grid, dim3(256), 0, s, g, a);
