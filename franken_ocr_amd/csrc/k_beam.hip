@@ -78,7 +78,7 @@ __device__ __forceinline__ uint32_t float_order(float v) { return static_cast<ui
 __device__ __forceinline__ uint32_t wave_bound(uint32_t mine, int W) {
     uint32_t bound = 0u;
 #pragma unroll
-    for (int bit = 31; bit >= 12; --bit) {
+    for (int bit = 31; bit >= 16; --bit) {
         const uint32_t t = bound | (1u << bit);
         if (__popcll(__ballot(mine >= t)) >= W) bound = t;
     }
@@ -108,15 +108,18 @@ __global__ __launch_bounds__(kThreads) void beam_scan_kernel(BeamSelect a, Parts
     const float none = __uint_as_float(0x7FC00000u);  // NaN: no logit
     float v[kPer];
     const int t0 = part * kChunk + static_cast<int>(threadIdx.x);
+    if ((part + 1) * kChunk <= a.vocab) {  // uniform
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) v[i] = t0 + i * kThreads < a.vocab ? x[t0 + i * kThreads] : none;
-    uint32_t banned = 0u;  // bit i: v[i] is
-    if (ban) {
-        uint32_t bw[kPer];
+        for (int i = 0; i < kPer; ++i) v[i] = x[t0 + i * kThreads];
+    } else {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) bw[i] = t0 + i * kThreads < a.vocab ? ban[(t0 + i * kThreads) >> 5] : 0u;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) banned |= (bw[i] >> (t0 & 31) & 1u) << i;  // kThreads keeps the bit's place
+        for (int i = 0; i < kPer; ++i) v[i] = t0 + i * kThreads < a.vocab ? x[t0 + i * kThreads] : none;
+    }
+    // the wave's words of the ban, one a lane: word 2 i + h is that of the tokens of v[i] in half h of the wave
+    uint32_t ban_word = 0u;
+    if (ban && lane < 2 * kPer) {
+        const int word = (part * kChunk + (lane >> 1) * kThreads + wave * 64 + (lane & 1) * 32) >> 5;
+        if (word < a.ban_words) ban_word = ban[word];
     }
     if (threadIdx.x == 0) s_n = 0;
     float most = -INFINITY;
@@ -126,19 +129,21 @@ __global__ __launch_bounds__(kThreads) void beam_scan_kernel(BeamSelect a, Parts
     // each wave sums relative to its own maximum, and they meet at the end; a
     // NaN's difference counts as -700, which adds nothing beside the maximum's 1
     double sum = 0.0;
-    if (m > -INFINITY) {
+    if (m > -INFINITY && m < INFINITY) {
+        const double dm = static_cast<double>(m);
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const double d = static_cast<double>(v[i]) - static_cast<double>(m);
-            sum += exp_below(v[i] == m ? 0.0 : d);
-        }
+        for (int i = 0; i < kPer; ++i) sum += exp_below(static_cast<double>(v[i]) - dm);
+    } else if (m == INFINITY) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) sum += v[i] == m ? 1.0 : 0.0;
     }
     sum = wave_sum_d_full(sum);
-    if (__any(banned)) {
+    if (__any(ban_word != 0u)) {
         most = -INFINITY;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            v[i] = banned >> i & 1u ? none : v[i];
+            const uint32_t w = __shfl(ban_word, 2 * i + (lane >> 5), 64);
+            v[i] = w >> (lane & 31) & 1u ? none : v[i];
             most = fmaxf(most, v[i]);
         }
     }
@@ -209,14 +214,16 @@ __global__ __launch_bounds__(kThreads) void beam_scan_kernel(BeamSelect a, Parts
             }
         }
     }
-    if (threadIdx.x == 0) {
+    if (wave == kWaves - 1) {  // a lane a wave's sum
         const float mx = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
-        double total = 0.0;
-        for (int o = 0; o < kWaves; ++o)
-            if (s_max[o] > -INFINITY)
-                total += s_sum[o] * exp_below(s_max[o] == mx ? 0.0 : static_cast<double>(s_max[o]) - static_cast<double>(mx));
-        q.max[to] = mx;
-        q.sum[to] = total;
+        const float mw = s_max[lane & (kWaves - 1)];
+        const double d = mw == mx ? 0.0 : static_cast<double>(mw) - static_cast<double>(mx);
+        const double mine = mw > -INFINITY ? s_sum[lane & (kWaves - 1)] * exp_below(d) : 0.0;
+        const double total = (readlane_d(mine, 0) + readlane_d(mine, 1)) + (readlane_d(mine, 2) + readlane_d(mine, 3));
+        if (lane == 0) {
+            q.max[to] = mx;
+            q.sum[to] = total;
+        }
     }
 }
 
@@ -239,7 +246,21 @@ __global__ __launch_bounds__(1024) void beam_pick_kernel(BeamSelect a, Parts q, 
     for (int i = t; i < W * W; i += blockDim.x) s_k[i] = 0ull;
     __syncthreads();
     for (int b = wave; wave < waves && b < W; b += waves) {
+        const size_t at = (row0 + b) * a.nparts;
+        uint64_t* keys = s_keys + static_cast<size_t>(wave) * a.nparts * W;
+        constexpr int kHeads = kBeamParts / 64;
+        // everything the row needs is requested before anything of it is used
         const double score = static_cast<double>(a.scores[row0 + b]);
+        float mp[kHeads];
+        double sp[kHeads];
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) {
+            const int p = lane + 64 * h;
+            mp[h] = p < a.nparts ? q.max[at + p] : -INFINITY;
+            sp[h] = p < a.nparts ? q.sum[at + p] : 0.0;
+        }
+#pragma unroll 4
+        for (int i = lane; i < a.nparts * W; i += 64) keys[i] = q.key[at * W + i];
         if (s_done[b]) {
             if (lane == 0) {
                 s_k[b * W] = (1ull << 32) | (0xFFFFFFFFull - a.eos);
@@ -248,29 +269,27 @@ __global__ __launch_bounds__(1024) void beam_pick_kernel(BeamSelect a, Parts q, 
             }
             continue;
         }
-        const size_t at = (row0 + b) * a.nparts;
-        uint64_t* keys = s_keys + static_cast<size_t>(wave) * a.nparts * W;
-        for (int i = lane; i < a.nparts * W; i += 64) keys[i] = q.key[at * W + i];
         float m = -INFINITY;
-        for (int p = lane; p < a.nparts; p += 64) m = fmaxf(m, q.max[at + p]);
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) m = fmaxf(m, mp[h]);
         m = wave_max_f_full(m);
         double sum = 0.0;
-        for (int p = lane; p < a.nparts; p += 64) {
-            const float mp = q.max[at + p];
-            if (mp > -INFINITY) sum += q.sum[at + p] * exp_below(mp == m ? 0.0 : static_cast<double>(mp) - static_cast<double>(m));
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) {
+            const double d = mp[h] == m ? 0.0 : static_cast<double>(mp[h]) - static_cast<double>(m);
+            sum += mp[h] > -INFINITY ? sp[h] * exp_below(d) : 0.0;
         }
         sum = wave_sum_d_full(sum);
         const double total = static_cast<double>(m) + log(sum);
         wave_lds_fence();
-        constexpr int kHeads = kBeamParts / 64;
         uint64_t head[kHeads];
-        int next[kHeads];
+        int left[kHeads];  // what a list holds behind its head
         uint64_t best = 0ull;
 #pragma unroll
         for (int h = 0; h < kHeads; ++h) {
             const int p = lane + 64 * h;
             head[h] = p < a.nparts ? keys[p * W] : 0ull;
-            next[h] = p * W + 1;
+            left[h] = W - 1;
             best = umax64(best, head[h]);
         }
         int n = 0;
@@ -284,8 +303,8 @@ __global__ __launch_bounds__(1024) void beam_pick_kernel(BeamSelect a, Parts q, 
 #pragma unroll
                 for (int h = 0; h < kHeads; ++h) {
                     if (head[h] == k) {
-                        head[h] = next[h] % W != 0 ? keys[next[h]] : 0ull;
-                        ++next[h];
+                        head[h] = left[h] > 0 ? keys[(lane + 64 * h) * W + W - left[h]] : 0ull;
+                        --left[h];
                     }
                     best = umax64(best, head[h]);
                 }
