@@ -43,6 +43,7 @@ int32_t entry(focr_hip_ctx* ctx, F body) noexcept {
     }
 }
 
+constexpr size_t kMaxLen = size_t(1) << 26;  // keeps every grid within 2^32 threads
 constexpr size_t kI32Max = static_cast<size_t>(std::numeric_limits<int32_t>::max());
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -66,6 +67,8 @@ int32_t tables_ok(const char* who, const focr_hip_paged* c, const uint32_t* tabl
     if (max_len > (max_pages << c->page_shift))
         return fail(FOCR_HIP_E_SHAPE, fmt("%s: max_len %zu exceeds max_pages * page_size %zu", who, max_len,
                                           max_pages << c->page_shift));
+    if (max_len > kMaxLen)
+        return fail(FOCR_HIP_E_SHAPE, fmt("%s: max_len %zu exceeds the gfx950 tier limit of %zu", who, max_len, kMaxLen));
     *t = PagedTables{tables, lens, static_cast<int>(n_seqs), max_pages, static_cast<uint32_t>(max_len)};
     return FOCR_HIP_OK;
 }
@@ -139,6 +142,10 @@ int32_t attend(focr_hip_ctx* ctx, const char* who, const focr_hip_paged* c, cons
     if (n_heads > 65535) return fail(FOCR_HIP_E_SHAPE, fmt("%s: n_heads %zu exceeds the gfx950 tier limit", who, n_heads));
     if (ldq < n_heads * c->head_dim || ldo < n_heads * c->head_dim || (step && ldkv < c->n_kv_heads * c->head_dim))
         return fail(FOCR_HIP_E_SHAPE, fmt("%s: a row stride is shorter than the row", who));
+    // the join's grid: a block to a head, and to each 256 keys at least of a key head
+    if (weights && c->n_kv_heads * (max_len / 256 + 65) > (size_t(1) << 24) - 1)
+        return fail(FOCR_HIP_E_SHAPE, fmt("%s: max_len %zu of %zu key heads exceeds the gfx950 tier limit with weights", who, max_len,
+                                          c->n_kv_heads));
     if (weights && ldw < max_len) return fail(FOCR_HIP_E_SHAPE, fmt("%s: ldw %zu is less than max_len %zu", who, ldw, max_len));
     if (step && max_len == 0) return fail(FOCR_HIP_E_SHAPE, fmt("%s: max_len is 0", who));
     if (!(scale >= 0.0f) || std::isinf(scale)) return fail(FOCR_HIP_E_ARG, fmt("%s: scale is not a positive number", who));
@@ -336,7 +343,8 @@ int32_t focr_hip_paged_evict(focr_hip_ctx* ctx, focr_hip_paged* c, const uint32_
             if ((st = k.end(who, "sequence"))) return st;
         }
         const size_t hist = paged_evict_hist_words(n_seqs * c->n_kv_heads, a.t.max_len, ctx->cu_count);
-        const size_t words = hist + (kept ? 0 : n_seqs * c->n_kv_heads * budget);
+        if (!kept) a.budget = static_cast<uint32_t>(std::max<size_t>(most, 1));  // more than max_len keeps no more
+        const size_t words = hist + (kept ? 0 : n_seqs * c->n_kv_heads * a.budget);
         a.kept = kept;
         if (words) {
             uint32_t* p = static_cast<uint32_t*>(ctx->scratch_get_capturable(kScrEvict, words * sizeof(uint32_t), who));
@@ -451,6 +459,9 @@ int32_t focr_hip_beam_reorder(focr_hip_ctx* ctx, size_t groups, size_t beams, co
         a.advance = advance != 0;
         for (size_t i = 0; i < n_caches; ++i) {
             if ((st = cache_ok(who, ctx, caches[i]))) return st;
+            for (size_t j = 0; j < i; ++j)
+                if (caches[i]->k == caches[j]->k || caches[i]->v == caches[j]->v)
+                    return fail(FOCR_HIP_E_ARG, fmt("beam_reorder: caches %zu and %zu are the same", j, i));
             if (caches[i]->page_shift != caches[0]->page_shift)
                 return fail(FOCR_HIP_E_SHAPE, "beam_reorder: caches of different page sizes share no tables");
         }
@@ -467,6 +478,8 @@ int32_t focr_hip_beam_reorder(focr_hip_ctx* ctx, size_t groups, size_t beams, co
         for (size_t i = 0; i < n_rings; ++i) {
             const focr_hip_rswa* c = rings[i];
             if (!c) return fail(FOCR_HIP_E_BAD_HANDLE, "null rswa cache");
+            for (size_t j = 0; j < i; ++j)
+                if (rings[j] == c) return fail(FOCR_HIP_E_ARG, fmt("beam_reorder: rings %zu and %zu are the same", j, i));
             if (c->ctx->device != ctx->device) return fail(FOCR_HIP_E_ARG, "beam_reorder: a ring cache of another device");
             if (c->n_streams != rows)
                 return fail(FOCR_HIP_E_SHAPE, fmt("beam_reorder: %zu streams for %zu rows", c->n_streams, rows));

@@ -464,11 +464,11 @@ int32_t focr_hip_paged_write(focr_hip_ctx* ctx, focr_hip_paged* cache, const flo
 /* One query row per sequence over its cache: q [n_seqs][n_heads * head_dim]
  * f32 (rows ldq floats apart), n_heads 1 .. 64 times n_kv_heads, query head h
  * reads key head h / (n_heads / n_kv_heads). Of the n = lens[s] keys (at most
- * max_len, which is what the call is sized for) it sees all (window 0), or the
+ * max_len <= 2^26, which is what the call is sized for) it sees all (window 0), or the
  * first min(prefix[s], n) (prefix null: none) and the last `window` — with the
  * prompt's length as prefix and a window of 128 what the R-SWA ring sees. out
  * [n_seqs][n_heads * head_dim] (rows ldo apart) = softmax(scale q.k) v, scale
- * 0 meaning 1 / sqrt(head_dim); zeros where there is no key. The sums are f32,
+ * not negative and 0 meaning 1 / sqrt(head_dim); zeros where there is no key. The sums are f32,
  * and the same call gives the same bits. weights (nullable)
  * [n_seqs][n_kv_heads][ldw], ldw >= max_len: every key that is seen has the
  * probabilities of its key head's query heads added. */

@@ -97,7 +97,8 @@ def _same(got, want, done, beams):
 
 
 @pytest.mark.parametrize("groups,beams,vocab", [(1, 1, 1), (1, 4, 129280), (3, 2, 4096), (2, 5, 4097), (2, 8, 50021),
-                                                (1, 32, 12289), (4, 3, 2), (2, 16, 7), (65, 1, 300), (1, 32, 8192)])
+                                                (1, 32, 12289), (4, 3, 2), (2, 16, 7), (65, 1, 300), (1, 32, 8192),
+                                                (1, 32, 129280), (1, 3, 524288), (1, 32, 524287)])
 def test_selection_against_64_bits(ctx, groups, beams, vocab):
     _say(f"select {groups} x {beams} over {vocab}")
     rng = np.random.default_rng(groups * 1000 + beams + vocab)
@@ -188,6 +189,7 @@ def test_refusals(ctx):
     from franken_ocr_amd.engine import PagedCache, RingCache, beam_reorder, beam_select
 
     E, S = _abi.FocrHipError, _abi.ContractViolation
+    twice = PagedCache(4, 16, 1, 64, ctx=ctx)
     f, u = lambda *s: ctx.empty(s, np.float32), lambda *s: ctx.to_device(np.zeros(s, np.uint32))  # noqa: E731
     for call, text in (
             (lambda: beam_select(f(33, 10), f(33), 33, u(33), u(33), f(33)), "beams 33"),
@@ -199,6 +201,8 @@ def test_refusals(ctx):
             (lambda: beam_reorder(u(4), 2, caches=[PagedCache(4, 16, 1, 64, ctx=ctx)]), "null"),
             (lambda: beam_reorder(u(4), 2, caches=[PagedCache(4, 16, 1, 64, ctx=ctx), PagedCache(4, 8, 1, 64, ctx=ctx)],
                                   tables=u(4, 2), lens=u(4)), "page sizes"),
+            (lambda: beam_reorder(u(4), 2, caches=[twice, twice], tables=u(4, 2), lens=u(4)), "are the same"),
+            (lambda: beam_select(f(2, 524289), f(2), 2, u(2), u(2), f(2)), "tier limit"),
             (lambda: beam_reorder(u(4), 2, rings=[RingCache(3, 8, ctx=ctx)]), "3 streams"),
             (lambda: beam_reorder(u(4), 2, rings=[RingCache(4, 8, ctx=ctx)]), "record_prefill")):
         with pytest.raises(E, match=text):

@@ -350,6 +350,78 @@ def test_scores_without_an_end(ctx):
         assert np.all(np.abs(got[s] - p @ v[:, 0]) <= tol)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_infinities_with_grouped_heads(ctx, dtype):
+    """Where q and the probabilities are split into terms: infinite keys (-inf scores), infinite values, NaN."""
+    _say(f"infinities, grouped, {dtype}")
+    rng = np.random.default_rng(14)
+    heads, dim = 5, 64
+    host = Host(rng, ctx, [100, 700, 100, 90, 40], 16, 1, dim, dtype)
+    q = np.abs(rng.standard_normal((5, heads * dim))).astype(np.float32) + 0.1
+    for s, keys in ((0, range(0, 100, 2)), (1, range(200, 700, 3)), (4, range(40))):
+        for j in keys:
+            host.k[host.tables[s, j // 16], 0, j % 16, 5] = -np.inf
+    host.v[host.tables[2, 1], 0, 3, 7] = np.inf    # sequence 2, key 19
+    host.v[host.tables[2, 2], 0, 1, 8] = -np.inf
+    host.k[host.tables[3, 5], 0, 9, 0] = np.nan    # sequence 3, key 89
+    host.dk.copy_from(_bits(host.k, dtype))
+    host.dv.copy_from(_bits(host.v, dtype))
+    dout = ctx.empty((5, heads * dim), np.float32)
+    host.cache.attention(ctx.to_device(q), host.dt, host.dl, dout)
+    got = dout.numpy().reshape(5, heads, dim)
+    assert np.all(np.isnan(got[3])) and np.all(np.isnan(got[4]))
+    for s in (0, 1, 2):
+        out, tol, _, _, _ = _attend_finite(host, s, q[s].reshape(heads, dim), host.lens[s])
+        if s == 2:
+            assert np.all(got[2, :, 7] == np.inf) and np.all(got[2, :, 8] == -np.inf)
+            out[:, 7:9], got[2, :, 7:9] = 0.0, 0.0
+            tol[:, 7:9] = 0.0
+        assert np.all(np.abs(got[s] - out) <= tol), s
+
+
+def _attend_finite(host, s, q, n):
+    """_attend over the keys without an infinite coordinate (the others' scores are -inf)."""
+    keys = np.arange(n)
+    k, v = host.rows(s, keys)
+    keys = keys[np.isfinite(k[:, 0]).all(axis=1)]
+    rows = host.rows
+
+    class Part:
+        kv = host.kv
+
+        def rows(self, s_, keys_):
+            kk, vv = rows(s_, keys[keys_])
+            return kk, np.where(np.isinf(vv), 0.0, vv)
+
+    return _attend(Part(), s, q, len(keys), 0, 0, 1.0 / np.sqrt(np.float32(q.shape[1])))
+
+
+@pytest.mark.parametrize("dtype,unit", [("f16", 2.0 ** -20), ("bf16", 2.0 ** -126), ("f32", 2.0 ** -126), ("bf16", 2.0 ** 100),
+                                        ("f16", 2.0 ** 12)])
+@pytest.mark.parametrize("heads", [1, 2, 8])
+def test_small_and_large_values(ctx, dtype, unit, heads):
+    """Caches whose values are subnormal, or large, in their type: products and sums in f32 as they are."""
+    _say(f"values of {unit} in {dtype}, {heads} heads")
+    rng = np.random.default_rng(15)
+    dim = 64
+    host = Host(rng, ctx, [150, 33], 16, 1, dim, dtype)
+    for s, n in enumerate(host.lens):
+        for j in range(n):
+            host.put(s, j, unit * rng.standard_normal((1, dim)), unit * rng.standard_normal((1, dim)))
+    host.dk.copy_from(_bits(host.k, dtype))
+    host.dv.copy_from(_bits(host.v, dtype))
+    q = (rng.standard_normal((2, heads * dim)) / unit).astype(np.float32)
+    if unit == 2.0 ** -126:
+        q = (rng.standard_normal((2, heads * dim)) * 2.0 ** 120).astype(np.float32)
+    dout = ctx.empty((2, heads * dim), np.float32)
+    host.cache.attention(ctx.to_device(q), host.dt, host.dl, dout)
+    got = dout.numpy().reshape(2, heads, dim)
+    for s, n in enumerate(host.lens):
+        out, tol, _, _, _ = _attend(host, s, q[s].reshape(heads, dim), n, 0, 0, 1.0 / np.sqrt(np.float32(dim)))
+        # besides: what a sum of subnormal f32 products rounds away, half of the least one a product or sum
+        assert np.all(np.abs(got[s] - out) <= tol + n * 2.0 ** -149), (s, float(np.abs(got[s] - out).max()))
+
+
 def test_far_offsets(ctx):
     """Pages past 2^32 bytes and 2^31 values of a pool."""
     _say("far offsets")
