@@ -142,8 +142,8 @@ int32_t attend(focr_hip_ctx* ctx, const char* who, const focr_hip_paged* c, cons
     if (n_heads > 65535) return fail(FOCR_HIP_E_SHAPE, fmt("%s: n_heads %zu exceeds the gfx950 tier limit", who, n_heads));
     if (ldq < n_heads * c->head_dim || ldo < n_heads * c->head_dim || (step && ldkv < c->n_kv_heads * c->head_dim))
         return fail(FOCR_HIP_E_SHAPE, fmt("%s: a row stride is shorter than the row", who));
-    // the join's grid: a block to a head, and to each 256 keys at least of a key head
-    if (weights && c->n_kv_heads * (max_len / 256 + 65) > (size_t(1) << 24) - 1)
+    // the join's grid: a block of up to 1024 threads to a head, and to 512 keys of a key head
+    if (weights && c->n_kv_heads * (max_len / 512 + 65) > (size_t(1) << 22) - 1)
         return fail(FOCR_HIP_E_SHAPE, fmt("%s: max_len %zu of %zu key heads exceeds the gfx950 tier limit with weights", who, max_len,
                                           c->n_kv_heads));
     if (weights && ldw < max_len) return fail(FOCR_HIP_E_SHAPE, fmt("%s: ldw %zu is less than max_len %zu", who, ldw, max_len));

@@ -178,7 +178,10 @@ __device__ __forceinline__ void join_waves(const PagedAttend& a, const float (*s
 // instruction, U of those for K and U for V in flight at once; a lane keeps
 // the same key's K and V, so the probabilities never leave their lanes, and
 // there is no barrier until the four waves' maxima, sums and outputs are
-// joined at the end.
+// joined at the end. Bound by HBM: 128 sequences of up to 16384 keys, 2 key
+// heads of 128 bf16, one query head each 204 us, 5.6 TB/s read (a large copy
+// moves 4.7); 64 sequences in f32, 64 wide, 107 us. Eight f32 rows in flight
+// for K and for V and four waves a SIMD are what the load latency takes.
 template <typename T, int D, int GT, int U>
 __global__ __launch_bounds__(256, GT == 1 ? 4 : 3) void paged_attend_kernel(PoolGeom g, PagedAttend a) {
     constexpr int E = Row16<T>::N;
@@ -352,6 +355,10 @@ __global__ __launch_bounds__(256, GT == 1 ? 4 : 3) void paged_attend_kernel(Pool
 // The running maximum is moved only where a score is well past it (any
 // reference gives the same quotient, and f32 holds the sums), so the usual
 // tile needs nothing from other lanes.
+// 128 sequences of up to 16384 keys, 16 heads on 2 key heads, bf16: 64 wide 119
+// us (4.8 TB/s), 128 wide 230 us (4.9); the f32 products alone took 134 and
+// 275. Loading a second tile ahead cost more waves than it hid latency (163
+// for 155 us then), as did two tiles at once (171 for 137).
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
@@ -663,25 +670,27 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_attend_mfma_kerne
 }
 
 // The splits of a row joined, out = sum_z acc_z f_z / sum_z l_z f_z with f_z =
-// exp2(m_z - max m), in the order of the splits within each of the 256 / (D /
+// exp2(m_z - max m), in the order of the splits within each of the NT / (D /
 // 4) groups of lanes, then over the groups.
-template <int D>
+template <int D, int NT>
 __device__ __forceinline__ void join_row(const PagedAttend& a, int h, int n_heads, int s, const uint4& e) {
     constexpr int L4 = D / 4;
-    constexpr int G = 256 / L4;
+    constexpr int G = NT / L4;
     __shared__ float4 s_acc[G][L4];
     __shared__ float s_l[G];
-    __shared__ float s_m[4];
+    __shared__ float s_m[NT / 64];
     const uint32_t nvis = e.x;
     const uint32_t keys = split_keys(nvis, a.nsplit, a.split_least);
     const int n = static_cast<int>((nvis + keys - 1) / keys);
     const size_t part = (static_cast<size_t>(s) * n_heads + h) * a.nsplit;
     float m = -INFINITY;
-    for (int z = threadIdx.x; z < n; z += 256) m = fmaxf(m, a.part_ml[part + z].x);
+    for (int z = threadIdx.x; z < n; z += NT) m = fmaxf(m, a.part_ml[part + z].x);
     m = wave_max_f_full(m);
     if ((threadIdx.x & 63) == 0) s_m[threadIdx.x >> 6] = m;
     __syncthreads();
-    m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+    m = s_m[0];
+#pragma unroll
+    for (int i = 1; i < NT / 64; ++i) m = fmaxf(m, s_m[i]);
     const float sf = m == -INFINITY ? 0.0f : m;
     const int gi = threadIdx.x / L4;
     const int d4 = threadIdx.x % L4;
@@ -718,6 +727,7 @@ __device__ __forceinline__ void join_row(const PagedAttend& a, int h, int n_head
 // weights[key] += sum over the key head's query heads of exp2(score - M) / L
 // for kWeightKeys keys from j0 on, M and L joined from the splits again.
 constexpr int kWeightKeys = 512;
+template <int NT>
 __device__ __forceinline__ void add_weights(const PagedAttend& a, int hk, int kv_heads, int s, const uint4& e, uint32_t j0) {
     __shared__ float2 s_ml[64];
     const uint32_t nvis = e.x;
@@ -725,7 +735,7 @@ __device__ __forceinline__ void add_weights(const PagedAttend& a, int hk, int kv
     const uint32_t keys = split_keys(nvis, a.nsplit, a.split_least);
     const int n = static_cast<int>((nvis + keys - 1) / keys);
     const size_t head0 = (static_cast<size_t>(s) * kv_heads + hk) * a.group;
-    for (int i = threadIdx.x >> 6; i < a.group; i += 4) {  // a wave a head
+    for (int i = threadIdx.x >> 6; i < a.group; i += NT / 64) {  // a wave a head
         const float2* ml = a.part_ml + (head0 + i) * a.nsplit;
         float m = -INFINITY, l = 0.0f;
         for (int z = threadIdx.x & 63; z < n; z += 64) m = fmaxf(m, ml[z].x);
@@ -737,7 +747,7 @@ __device__ __forceinline__ void add_weights(const PagedAttend& a, int hk, int kv
     }
     __syncthreads();
     const uint32_t end = min(j0 + kWeightKeys, nvis);
-    for (uint32_t j = j0 + threadIdx.x; j < end; j += 256) {
+    for (uint32_t j = j0 + threadIdx.x; j < end; j += NT) {
         float w = 0.0f;
         for (int i = 0; i < a.group; ++i)
             w += __builtin_amdgcn_exp2f(a.scores[(head0 + i) * a.score_ld + j] - s_ml[i].x) / s_ml[i].y;
@@ -749,17 +759,17 @@ __device__ __forceinline__ void add_weights(const PagedAttend& a, int hk, int kv
 // Grid (head, then chunk of keys x key head where weights are gathered;
 // sequence). The lengths are read from what the splits' launch noted: a step
 // counts them up here.
-template <int D>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttend a, int kv_heads) {
+template <int D, int NT>
+__global__ __launch_bounds__(NT) void paged_join_kernel(PagedAttend a, int kv_heads) {
     const int s = blockIdx.y;
     const uint4 e = a.seen[s];
     if (e.x == kPagedNone) return;
     const int n_heads = kv_heads * a.group;
     const int b = static_cast<int>(blockIdx.x) - n_heads;
     if (b < 0)
-        join_row<D>(a, blockIdx.x, n_heads, s, e);
+        join_row<D, NT>(a, blockIdx.x, n_heads, s, e);
     else
-        add_weights(a, b % kv_heads, kv_heads, s, e, static_cast<uint32_t>(b / kv_heads) * kWeightKeys);
+        add_weights<NT>(a, b % kv_heads, kv_heads, s, e, static_cast<uint32_t>(b / kv_heads) * kWeightKeys);
 }
 
 // Rows of k / v [rows][kv_heads * D] into the slots (seq, pos) of the cache;
@@ -1199,12 +1209,21 @@ void attend(hipStream_t s, const focr_hip_paged* c, const PagedAttend& a) {
     const PoolGeom g = geom_of(c);
     const int kv = static_cast<int>(c->n_kv_heads);
     const auto grid = [&](int gt) { return dim3(a.nsplit, kv * ((a.group + gt - 1) / gt), a.t.n_seqs); };
+    // By query heads to a key head, 128 sequences of up to 16384 keys on 2 key
+    // heads, VALU kernel / matrix cores: bf16 128 wide, one 214 / 223 us, two
+    // 223 / 225, three 248 / 227, four 253 / 228; 64 wide 112 / 132, 117 / 133,
+    // 133 / 135, 136 / 135; f32 64 wide, 64 sequences, two 122 / 136, four 142 / 138.
     if (a.group > 2)
         FOCR_LAUNCH((paged_attend_mfma_kernel<T, D>), grid(16), dim3(256), 0, s, g, a);
     else if (a.group == 2)
         FOCR_LAUNCH((paged_attend_kernel<T, D, 2, 8>), grid(2), dim3(256), 0, s, g, a);
     else
         FOCR_LAUNCH((paged_attend_kernel<T, D, 1, 8>), grid(1), dim3(256), 0, s, g, a);
+}
+
+template <int D, int NT>
+void launch_join(hipStream_t s, dim3 grid, const PagedAttend& a, int kv) {
+    FOCR_LAUNCH((paged_join_kernel<D, NT>), grid, dim3(NT), 0, s, a, kv);
 }
 
 template <typename T>
@@ -1239,12 +1258,14 @@ hipError_t launch_paged_attend(hipStream_t s, const focr_hip_paged* c, const Pag
     ProfScope ps(ctx, "paged_join");
     const uint32_t chunks = a.weights ? (a.t.max_len + kWeightKeys - 1) / kWeightKeys : 0;
     const dim3 grid(kv * (a.group + chunks), a.t.n_seqs);
+    // 1024 threads where a row has many splits to join (64 rows of 256 splits: 10 -> 7.5 us)
+    const bool many = a.nsplit > 64;
     if (c->head_dim == 64)
-        FOCR_LAUNCH(paged_join_kernel<64>, grid, dim3(256), 0, s, a, kv);
+        many ? launch_join<64, 1024>(s, grid, a, kv) : launch_join<64, 256>(s, grid, a, kv);
     else if (c->head_dim == 128)
-        FOCR_LAUNCH(paged_join_kernel<128>, grid, dim3(256), 0, s, a, kv);
+        many ? launch_join<128, 1024>(s, grid, a, kv) : launch_join<128, 256>(s, grid, a, kv);
     else
-        FOCR_LAUNCH(paged_join_kernel<256>, grid, dim3(256), 0, s, a, kv);
+        many ? launch_join<256, 1024>(s, grid, a, kv) : launch_join<256, 256>(s, grid, a, kv);
     return hipGetLastError();
 }
 
@@ -1267,9 +1288,14 @@ hipError_t launch_paged_write(hipStream_t s, const focr_hip_paged* c, const floa
     return hipGetLastError();
 }
 
+// A block to a row keeps up to 16384 keys in registers and reads longer rows in
+// every pass; a block to a tile takes four dependent launches. Whole evictions,
+// block to a row / to a tile, us: 10 rows of 12000 slots 25 / 30, of 20000 44 /
+// 32, of 33000 62 / 34; 80 rows 27 / 34, 46 / 35, 64 / 48; 240 rows 35 / 57,
+// 54 / 70, 74 / 91.
 size_t paged_evict_hist_words(size_t rows, uint32_t max_len, int cu_count) {
     const size_t tiles = (static_cast<size_t>(max_len) + kLongTile - 1) / kLongTile;
-    return tiles > 1 && rows < static_cast<size_t>(cu_count) ? rows * (4 + tiles * (2 + 3 * kBins)) : 0;
+    return max_len > 16 * kSelThreads && 2 * rows <= static_cast<size_t>(cu_count) ? rows * (4 + tiles * (2 + 3 * kBins)) : 0;
 }
 
 hipError_t launch_paged_evict(hipStream_t s, const focr_hip_paged* c, const PagedEvict& a, focr_hip_ctx* ctx) {

@@ -65,11 +65,14 @@ FOCR_INDEX uint32_t split_keys(uint32_t nvis, int nsplit, uint32_t least) {
 }
 
 // Splits of a call whose sequences see up to max_seen keys: as many as give
-// every CU twelve blocks were all that long, of at most kPagedChunkMax keys (their
-// rows are kept in LDS). Sequences that are shorter get fewer splits of the
-// same length, so that blocks are alike (ragged lengths: equal counts of
-// unequal splits left CUs idle a quarter of the time); but where a window hides
-// most of what max_seen counts, what is seen is divided by the count.
+// every CU twelve blocks were all that long, of at most kPagedChunkMax keys.
+// Sequences that are shorter get fewer splits of the same length, so that
+// blocks are alike (equal counts of unequal splits left CUs idle a quarter of
+// the time where lengths are ragged); but where a window hides most of what
+// max_seen counts, what is seen is divided by the count. Blocks a CU at 6 / 12 /
+// 32, us: 16 sequences x 10 heads of up to 4096 keys 53 / 49 / 51; 2 x 8 heads
+// of up to 131071 171 / 171 / 184; 24 x 10 windowed 27 / 28 / 32. At most 2048 /
+// 512 / 256 keys: 128 x 2 heads of up to 16384 keys 132 / 119 / 127.
 inline PagedSplits pick_splits(size_t n_seqs, size_t kv_heads, int group, uint32_t max_seen, bool window, int cu_count) {
     const uint64_t rows = n_seqs * kv_heads * static_cast<uint64_t>((group + 15) / 16);
     const uint64_t unit = kPagedChunkUnit;

@@ -32,9 +32,11 @@ HEAD_DIM = 128
 RING_WINDOW = 128
 
 
-def _p(x) -> C.c_void_p:
-    if x is None:
-        return C.c_void_p()
+def _p(x) -> C.c_void_p | None:
+    if type(x) is DeviceArray:
+        return x._p
+    if x is None:  # a null pointer
+        return None
     if isinstance(x, DeviceArray):
         return x.c_ptr
     if isinstance(x, np.ndarray):
@@ -417,14 +419,15 @@ class PagedCache:
 
     def _heads(self, who: str, q: DeviceArray, out: DeviceArray, n: int, n_heads, ldq, ldo):
         heads = n_heads if n_heads is not None else q.shape[-1] // self.head_dim
-        for name, a, ld in (("q", q, ldq), ("out", out, ldo)):
-            self._fits(who, name, a, n, heads * self.head_dim, ld)
-        return heads, ldq or heads * self.head_dim, ldo or heads * self.head_dim
+        row = heads * self.head_dim
+        self._fits(who, "q", q, n, row, ldq)
+        self._fits(who, "out", out, n, row, ldo)
+        return heads, ldq or row, ldo or row
 
     @staticmethod
-    def _fits(who: str, name: str, a, rows: int, wide: int, ld) -> None:
-        """The array holds `rows` rows of `wide` values, `ld` apart (a raw pointer is taken on trust)."""
-        if isinstance(a, DeviceArray) and rows and a.nbytes // a.dtype.itemsize < (rows - 1) * (ld or wide) + wide:
+    def _fits(who: str, name: str, a, rows: int, wide: int, ld=None, size: int = 4) -> None:
+        """The array holds `rows` rows of `wide` values of `size` bytes, `ld` apart (a raw pointer is taken on trust)."""
+        if type(a) is DeviceArray and rows and a.nbytes < size * ((rows - 1) * (ld or wide) + wide):
             raise _abi.ContractViolation(_abi.E_SHAPE, f"{who}: {name} of shape {a.shape} holds no {rows} rows of {wide}")
 
     def write(self, k: DeviceArray, v: DeviceArray, pos: DeviceArray, tables: DeviceArray,
@@ -435,7 +438,7 @@ class PagedCache:
         rows, row = pos.shape[0], self.n_kv_heads * self.head_dim
         self._fits("paged_write", "k", k, rows, row, ldkv)
         self._fits("paged_write", "v", v, rows, row, ldkv)
-        self._fits("paged_write", "seq", seq, rows, 1, None)
+        self._fits("paged_write", "seq", seq, rows, 1)
         _abi.call("focr_hip_paged_write", self.ctx.handle, self._h, _p(k), _p(v), ldkv or row, rows, _p(seq), _p(pos),
                   _p(tables), n, wide, 1 if check else 0)
 
@@ -449,7 +452,7 @@ class PagedCache:
         >= max_len] gathers the probabilities."""
         n, wide = self._rows("paged_attention", tables, lens)
         heads, ldq, ldo = self._heads("paged_attention", q, out, n, n_heads, ldq, ldo)
-        self._fits("paged_attention", "prefix", prefix, n, 1, None)
+        self._fits("paged_attention", "prefix", prefix, n, 1)
         ldw = self._weights("paged_attention", weights, n)
         _abi.call("focr_hip_paged_attention", self.ctx.handle, self._h, _p(q), ldq, heads, _p(tables), n, wide, _p(lens),
                   wide * self.page_size if max_len is None else int(max_len), _p(prefix), int(window), float(scale),
@@ -466,7 +469,7 @@ class PagedCache:
         row = self.n_kv_heads * self.head_dim
         self._fits("paged_step", "k_steps", k_steps, n, row, ldkv)
         self._fits("paged_step", "v_steps", v_steps, n, row, ldkv)
-        self._fits("paged_step", "prefix", prefix, n, 1, None)
+        self._fits("paged_step", "prefix", prefix, n, 1)
         ldw = self._weights("paged_step", weights, n)
         _abi.call("focr_hip_paged_step", self.ctx.handle, self._h, _p(q), ldq, heads, _p(k_steps), _p(v_steps),
                   ldkv or row, _p(tables), n, wide, _p(lens), wide * self.page_size if max_len is None else int(max_len),
@@ -491,8 +494,8 @@ class PagedCache:
         most = wide * self.page_size if max_len is None else int(max_len)
         ldw = self._weights("paged_evict", weights, n)
         dst_ldw = self._weights("paged_evict", dst_weights, n)
-        self._fits("paged_evict", "dst_lens", dst_lens, n, 1, None)
-        self._fits("paged_evict", "kept", kept, n * self.n_kv_heads, int(budget), None)
+        self._fits("paged_evict", "dst_lens", dst_lens, n, 1)
+        self._fits("paged_evict", "kept", kept, n * self.n_kv_heads, int(budget))
         if dst_tables.shape[0] < n:
             raise _abi.ContractViolation(_abi.E_SHAPE, f"paged_evict: dst_tables of shape {dst_tables.shape} for {n} rows")
         _abi.call("focr_hip_paged_evict", self.ctx.handle, self._h, _p(tables), n, wide, _p(lens),
@@ -525,11 +528,14 @@ def beam_select(logits: DeviceArray, scores: DeviceArray, beams: int, parents: D
     beams = int(beams)
     if beams <= 0 or rows % beams:
         raise _abi.ContractViolation(_abi.E_SHAPE, f"beam_select: {rows} rows are no groups of {beams}")
+    fits = PagedCache._fits
     for name, a in (("scores", scores), ("parents", parents), ("tokens", tokens), ("new_scores", new_scores),
-                    ("done", done), ("new_done", new_done), ("history_len", history_len)):
-        PagedCache._fits("beam_select", name, a, rows, 1, None)
+                    ("history_len", history_len)):
+        fits("beam_select", name, a, rows, 1)
+    fits("beam_select", "done", done, rows, 1, size=1)
+    fits("beam_select", "new_done", new_done, rows, 1, size=1)
     cap = history.shape[1] if history is not None else 0
-    PagedCache._fits("beam_select", "history", history, rows, cap, None)
+    fits("beam_select", "history", history, rows, cap)
     nw = whitelist.shape[0] if whitelist is not None else 0
     _abi.call("focr_hip_beam_select", logits.ctx.handle, _p(logits), vocab, rows // beams, beams, vocab, _p(scores),
               _p(done), int(eos), _p(history), cap, _p(history_len), int(ngram_size), int(window), _p(whitelist), nw,
@@ -547,17 +553,19 @@ def beam_reorder(parents: DeviceArray, beams: int, tokens: DeviceArray | None = 
     rows, beams = parents.shape[0], int(beams)
     if beams <= 0 or rows % beams:
         raise _abi.ContractViolation(_abi.E_SHAPE, f"beam_reorder: {rows} rows are no groups of {beams}")
-    for name, a in (("tokens", tokens), ("history_len", history_len), ("lens", lens)):
-        PagedCache._fits("beam_reorder", name, a, rows, 1, None)
+    fits = PagedCache._fits
+    fits("beam_reorder", "tokens", tokens, rows, 1)
+    fits("beam_reorder", "history_len", history_len, rows, 1)
+    fits("beam_reorder", "lens", lens, rows, 1)
     cap = history.shape[1] if history is not None else 0
     wide = tables.shape[1] if tables is not None else 0
-    PagedCache._fits("beam_reorder", "history", history, rows, cap, None)
-    PagedCache._fits("beam_reorder", "tables", tables, rows, wide, None)
-    paged = (C.c_void_p * len(caches))(*[c._h.value for c in caches])
-    ring = (C.c_void_p * len(rings))(*[c._h.value for c in rings])
+    fits("beam_reorder", "history", history, rows, cap)
+    fits("beam_reorder", "tables", tables, rows, wide)
+    paged = (C.c_void_p * len(caches))(*[c._h.value for c in caches]) if caches else None
+    ring = (C.c_void_p * len(rings))(*[c._h.value for c in rings]) if rings else None
     _abi.call("focr_hip_beam_reorder", parents.ctx.handle, rows // beams, beams, _p(parents), _p(tokens), _p(history),
-              cap, _p(history_len), 1 if advance else 0, C.cast(paged, C.c_void_p), len(caches), _p(tables), wide,
-              _p(lens), C.cast(ring, C.c_void_p), len(rings), 1 if check else 0)
+              cap, _p(history_len), 1 if advance else 0, paged, len(caches), _p(tables), wide, _p(lens), ring,
+              len(rings), 1 if check else 0)
 
 
 def prefill_chunk_bounds(seq: int, chunk: int) -> list:
