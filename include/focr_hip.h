@@ -497,9 +497,9 @@ int32_t focr_hip_paged_step(focr_hip_ctx* ctx, focr_hip_paged* cache, const floa
  * may read and no two share (source pages may be shared, so nothing moves
  * within them). dst_lens [n_seqs] = min(n, budget); dst_weights
  * [n_seqs][n_kv_heads][dst_ldw] the weights of the slots that stay; kept
- * (nullable) [n_seqs][n_kv_heads][budget] their slots. dst_lens may be lens.
- * With several layers each has weights, so evicts, of its own; the lengths
- * agree. */
+ * (nullable) [n_seqs][n_kv_heads][budget] their slots. With several layers
+ * each has weights, so evicts, of its own, and the new lengths agree; dst_lens
+ * may be lens in the last of the calls that read it. */
 int32_t focr_hip_paged_evict(focr_hip_ctx* ctx, focr_hip_paged* cache, const uint32_t* tables, size_t n_seqs,
                              size_t max_pages, const uint32_t* lens, size_t max_len, const float* weights,
                              size_t ldw, size_t budget, size_t sinks, size_t recent,

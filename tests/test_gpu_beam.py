@@ -12,7 +12,9 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from franken_ocr_amd import _abi
+from franken_ocr_amd import _abi, synth
+from test_gpu_decoder import _device as _decoder
+from test_gpu_decoder import model  # noqa: F401 (a fixture)
 from test_gpu_paged import Host, _capture
 
 pytestmark = pytest.mark.gpu
@@ -412,6 +414,57 @@ def test_beam_search_over_pages_and_rings(ctx):
         assert history.numpy()[:, : i + 1].tolist() == texts
     assert mixed > steps // 3
     assert lens.numpy().tolist() == np.repeat([x + steps for x in prompts], beams).tolist()
+
+
+def test_beam_search_over_the_decoder(ctx, model):  # noqa: F811
+    """Decoder.step, beam_select and beam_reorder of its rings: each beam's text, fed to fresh caches token by token,
+    has the score that the search gave it. A row of the decoder is the same whatever the other rows are, so the logits
+    are the same bits; a score is rounded to f32 once a step, at most half a unit of its place each time."""
+    _say("search over the decoder")
+    from franken_ocr_amd.engine import RingCache, beam_reorder, beam_select
+
+    H, V, G, beams, steps = 1280, 4096, 24, 3, 7
+    layers, _, dec = _decoder(ctx, model)
+    kv = [[ctx.to_device(synth.f32_normal(synth.seed_of(24000 + 2 * n + i), 10 * G * 128)) for i in (0, 1)] for n in range(3)]
+    emb = synth.f32_normal(synth.seed_of(24100), V * H).reshape(V, H)
+
+    def fresh():
+        caches = []
+        for k, v in kv:
+            c = RingCache(beams, G, ctx=ctx)
+            for s in range(beams):
+                c.record_prefill(s, k, v, G)
+            caches.append(c)
+        return caches
+
+    caches = fresh()
+    logits, greedy = ctx.empty((beams, V), np.float32), ctx.empty((beams,), np.uint32)
+    scores = ctx.to_device(np.array([0.0, -np.inf, -np.inf], np.float32))
+    p, t = ctx.empty((beams,), np.uint32), ctx.empty((beams,), np.uint32)
+    history, size = ctx.to_device(np.zeros((beams, steps), np.uint32)), ctx.to_device(np.zeros(beams, np.uint32))
+    tokens, moved = np.full(beams, 5), 0
+    for i in range(steps):
+        dec.step(caches, np.full(beams, G + i, np.uint32), ctx.to_device(emb[tokens]), greedy, logits)
+        if i == 0:  # a beam of one is the greedy step
+            one = [ctx.empty((1,), np.uint32) for _ in "pt"]
+            beam_select(logits.view_rows(0, 1), ctx.to_device(np.zeros(1, np.float32)), 1, *one, ctx.empty((1,), np.float32))
+            assert one[1].numpy()[0] == greedy.numpy()[0]
+        beam_select(logits, scores, beams, p, t, scores, history=history, history_len=size, ngram_size=2, window=0, eos=V)
+        beam_reorder(p, beams, tokens=t, history=history, history_len=size, advance=True, rings=caches, check=True)
+        tokens = t.numpy()
+        moved += int(np.any(p.numpy() != np.arange(beams)))
+    texts, got = history.numpy(), scores.numpy()
+    assert moved > 0 and len({tuple(x) for x in texts.tolist()}) == beams
+    assert np.all(np.diff(got) <= 0)
+    again, feed, want = fresh(), np.full(beams, 5), np.zeros(beams)
+    for i in range(steps):
+        dec.step(again, np.full(beams, G + i, np.uint32), ctx.to_device(emb[feed]), greedy, logits)
+        x = logits.numpy().astype(np.float64)
+        m = x.max(axis=1)
+        total = m + np.log(np.exp(x - m[:, None]).sum(axis=1))
+        feed = texts[:, i]
+        want += x[np.arange(beams), feed] - total
+    assert np.all(np.abs(got - want) <= steps * (2.0 ** -24 * np.abs(want) + 1e-9)), (got, want)
 
 
 def test_captured_beam_step_replays(ctx):
