@@ -779,6 +779,7 @@ hipError_t launch_clear_words(hipStream_t s, uint32_t* p, size_t n);
 // states of the chosen beams put where their slots are.
 constexpr int kBeamMax = 32;
 constexpr int kBeamParts = 128;  // chunks of a row at most
+constexpr int kBeamBanSpan = 256;  // a thread of the scan's blocks to a token
 struct BeamSelect {
     const float* logits;  // [groups * beams][ld]
     size_t ld;
@@ -788,6 +789,13 @@ struct BeamSelect {
     uint32_t eos;
     const uint32_t* ban_bits;  // nullable, [groups * beams][ban_words]
     int ban_words;
+    // or, where the ban looks at no more than kBeamBanSpan tokens, what it is
+    // found from inside the scan (ngram 0: not so)
+    const uint32_t* history;
+    const uint32_t* history_len;
+    int cap, ngram, window;
+    const uint32_t* whitelist;
+    int n_white;
     uint32_t* parents;
     uint32_t* tokens;
     float* new_scores;

@@ -394,7 +394,17 @@ int32_t focr_hip_beam_select(focr_hip_ctx* ctx, const float* logits, size_t ld, 
         a.nparts = beam_parts(a.vocab);
         a.part = ctx->scratch_get_capturable(kScrBeam, beam_part_bytes(static_cast<int>(rows), a.beams, a.nparts), who);
         if (!a.part) return no_scratch(ctx);
-        if (ngram_size) {
+        // what the ban looks at; a thread a token finds it inside the scan (check = 1 needs the flags of the launch before)
+        const size_t span = window ? std::min(window, history_cap) : history_cap;
+        if (ngram_size && span <= static_cast<size_t>(kBeamBanSpan) && !check) {
+            a.history = history;
+            a.history_len = history_len;
+            a.cap = static_cast<int>(history_cap);
+            a.ngram = static_cast<int>(ngram_size);
+            a.window = static_cast<int>(window);
+            a.whitelist = whitelist;
+            a.n_white = static_cast<int>(n_whitelist);
+        } else if (ngram_size) {
             const size_t words = (vocab + 31) / 32;
             SamplerArgs p{};
             p.history = history;

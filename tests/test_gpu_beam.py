@@ -145,9 +145,10 @@ def test_selection_of_odd_rows(ctx):
     _same(got, _select(x, scores, beams, done, [set()] * 40), done, beams)
 
 
-@pytest.mark.parametrize("n,window,white", [(2, 0, []), (3, 64, [5, 9]), (1, 20, []), (35, 128, [])])
-def test_selection_with_the_ngram_ban(ctx, n, window, white):
-    _say(f"ban n={n} window={window}")
+@pytest.mark.parametrize("check", [True, False])  # the ban found by a launch of its own, or by the scan where it is short
+@pytest.mark.parametrize("n,window,white", [(2, 0, []), (3, 64, [5, 9]), (1, 20, []), (35, 128, []), (1, 0, [3]), (200, 0, [])])
+def test_selection_with_the_ngram_ban(ctx, n, window, white, check):
+    _say(f"ban n={n} window={window} check={check}")
     rng = np.random.default_rng(n)
     groups, beams, vocab, cap = 3, 4, 5000, 200
     rows = groups * beams
@@ -165,11 +166,28 @@ def test_selection_with_the_ngram_ban(ctx, n, window, white):
     scores = (-rng.random(rows)).astype(np.float32)
     done = np.zeros(rows, np.uint8)
     kw = dict(ngram_size=n, window=window, whitelist=ctx.to_device(np.array(white, np.uint32)) if white else None)
-    got = _run(ctx, x, scores, beams, done, history, lens, **kw)
-    assert sum(map(len, banned)) > 0
+    got = _run(ctx, x, scores, beams, done, history, lens, check=check, **kw)
+    assert n == 200 or sum(map(len, banned)) > 0
     _same(got, _select(x, scores, beams, done, banned), done, beams)
     with pytest.raises(_abi.ContractViolation, match="history_len"):
         _run(ctx, x, scores, beams, done, history, [cap + 1] * rows, **kw)
+
+
+@pytest.mark.parametrize("cap,window", [(256, 0), (257, 0), (700, 256), (700, 257), (700, 0)])
+def test_ban_of_short_and_long_spans(ctx, cap, window):
+    """Both ways of finding the ban, on either side of what the scan's blocks take, over several chunks of a row."""
+    _say(f"ban cap={cap} window={window}")
+    rng = np.random.default_rng(cap + window)
+    rows, beams, vocab = 6, 3, 9000
+    lens = [cap, cap - 1, 2, 300 if cap > 300 else 200, 1, 0]
+    history = rng.integers(0, 30, (rows, cap)).astype(np.uint32) * 300  # tokens of every chunk
+    x = rng.standard_normal((rows, vocab)).astype(np.float32)
+    x[:, ::300] += 8
+    banned = [_bans(history[r, :lens[r]].tolist(), 2, window) for r in range(rows)]
+    assert sum(map(len, banned)) > 10
+    scores, done = (-rng.random(rows)).astype(np.float32), np.zeros(rows, np.uint8)
+    got = _run(ctx, x, scores, beams, done, history, lens, check=False, ngram_size=2, window=window)
+    _same(got, _select(x, scores, beams, done, banned), done, beams)
 
 
 def test_selection_in_place(ctx):
