@@ -89,7 +89,8 @@ __device__ __forceinline__ uint32_t wave_bound(uint32_t mine, int W) {
 // n - 1 tokens are the last n - 1 bans the token behind it) as bits of the chunk
 // from token t0 on, by the scan's own blocks: a window of up to a thread a token
 // lies in LDS. A launch that finds the ban beforehand takes 4 us and the wait
-// here 1.6 to 3.2: a step of 1 x 4 beams 19.9 -> 16.8 us, of 8 x 8 103 and 104. Returns how many tokens the ban looked at.
+// here 1.6 to 3.2: a step of 1 x 4 beams 19.9 -> 16.8 us, of 8 x 8 103 and 104.
+// Returns how many tokens the ban looked at.
 __device__ __forceinline__ int ban_chunk(const BeamSelect& a, int row, uint32_t raw_len, int t0, uint32_t* s_seq, uint32_t* s_ban) {
     const int L = raw_len > static_cast<uint32_t>(a.cap) ? a.cap : static_cast<int>(raw_len);
     const int start = a.window != 0 && L > a.window ? L - a.window : 0;
