@@ -347,11 +347,17 @@ __global__ __launch_bounds__(256, GT == 1 ? 4 : 3) void paged_attend_kernel(Pool
 // An f32 cache runs v_mfma_f32_16x16x4_f32. A 16-bit cache's K and V are exact
 // operands of the 16-bit instructions (16x16x32 for the scores, 16x16x16 for
 // the output, at eight and four times the f32 rate); q and P are f32 and are
-// written as sums of 16-bit terms that hold their 24 bits: three of bf16, cut
-// off (exact), or two of f16, rounded (to 2^-23), after q's row is scaled by a
-// power of two to below 2^15 and P by 2^14, so that f16's exponents reach.
-// The terms do not hold infinities (an infinite K times a term that is zero is
-// NaN): a wave whose sums come out not finite does its keys again in f32.
+// written as sums of 16-bit terms: three of bf16, cut off (exact), or two of
+// f16, rounded. q's row is scaled by a power of two to below 2^15 and P by 2^14;
+// the second f16 term is what the first leaves, times 2^12, with sums of its
+// own: for values from 2^-14 on, the first is a normal number and the second
+// holds the rest to 2^-23 of the value (unscaled, it would be subnormal below
+// 2^-2). Values below 2^-14 have no such terms, and infinities have none in
+// either type (an infinite K times a term that is zero is NaN): a wave that
+// meets a smaller coordinate of q or probability (2^-28 of the reference's), or
+// whose sums come out not finite, does its keys in f32 products instead. In f16
+// that costs where scores are far apart: 120 us as below, 144 to 153 where most
+// waves meet such a probability, 134 with the f32 products alone.
 // The running maximum is moved only where a score is well past it (any
 // reference gives the same quotient, and f32 holds the sums), so the usual
 // tile needs nothing from other lanes.
@@ -370,7 +376,7 @@ template <typename T>
 struct Terms {  // f32: its own products alone
     static constexpr bool kSplit = false;
     static constexpr int N = 1;
-    static constexpr float kTop = 0.0f, kPast = 8.0f;
+    static constexpr float kTop = 0.0f, kPast = 8.0f, kLeast = 0.0f, kApart = 1.0f;
     static __device__ void split2(float, float, uint32_t*) {}
     static __device__ v4f scores(const u4&, const u4&, v4f c) { return c; }
     static __device__ v4f output(const u2&, const u2&, v4f c) { return c; }
@@ -381,6 +387,8 @@ struct Terms<__bf16> {
     static constexpr int N = 3;
     static constexpr float kTop = 0.0f;   // the maximum's exponential is 2^kTop
     static constexpr float kPast = 8.0f;  // how far a score may pass the reference
+    static constexpr float kLeast = 0.0f;  // the least value that the terms hold
+    static constexpr float kApart = 1.0f;  // what the later terms are scaled by
     // two values' terms in one word each
     static __device__ __forceinline__ void split2(float x, float y, uint32_t* w) {
 #pragma unroll
@@ -404,13 +412,15 @@ struct Terms<_Float16> {
     static constexpr int N = 2;
     static constexpr float kTop = 14.0f;
     static constexpr float kPast = 15.0f;
+    static constexpr float kLeast = 0x1p-14f;
+    static constexpr float kApart = 0x1p12f;
     static __device__ __forceinline__ void split2(float x, float y, uint32_t* w) {
 #pragma unroll
         for (int t = 0; t < N; ++t) {
             const _Float16 a = static_cast<_Float16>(x), b = static_cast<_Float16>(y);
             w[t] = __builtin_bit_cast(uint16_t, a) | static_cast<uint32_t>(__builtin_bit_cast(uint16_t, b)) << 16;
-            x -= static_cast<float>(a);
-            y -= static_cast<float>(b);
+            x = (x - static_cast<float>(a)) * kApart;
+            y = (y - static_cast<float>(b)) * kApart;
         }
     }
     static __device__ __forceinline__ v4f scores(const u4& k, const u4& q, v4f c) {
@@ -421,6 +431,9 @@ struct Terms<_Float16> {
     }
 };
 
+// A number's magnitude as a whole number of the same order, zero the greatest.
+__device__ __forceinline__ uint32_t size_order(float v) { return (__float_as_uint(v) & 0x7FFFFFFFu) - 1u; }
+
 template <typename T, int D>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_attend_mfma_kernel(PoolGeom g, PagedAttend a) {
     using TT = Terms<T>;
@@ -429,7 +442,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_attend_mfma_kerne
     constexpr int KC = C / 4;                // K pieces of a lane
     constexpr int VE = C >= 16 ? E : E / 2;  // values of a V piece (8 bytes where a row has 8 pieces of 16)
     constexpr int VC = D / (16 * VE);        // V pieces of a lane and key
-    __shared__ uint32_t s_row[kPagedChunkMax];
+    __shared__ __align__(16) uint32_t s_row[kPagedChunkMax];
     __shared__ float s_acc[4][16][D];
     __shared__ float2 s_ml[4][16];
     const int z = blockIdx.x;
@@ -470,8 +483,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_attend_mfma_kerne
             return *reinterpret_cast<const u4*>(p);
         }
     };
-    const auto run = [&](auto f32_products) {
+    // false where a value has no terms: the sums are of no use then
+    const auto run = [&](auto f32_products) -> bool {
         constexpr bool EXACT = decltype(f32_products)::value;
+        constexpr bool APART = !EXACT && TT::kApart != 1.0f;
         m = -INFINITY;
         l = 0.0f;
 #pragma unroll
@@ -504,6 +519,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_attend_mfma_kerne
                 for (int c = 0; c < KC; ++c)
 #pragma unroll
                     for (int j = 0; j < E; ++j) q[c][j] *= by;
+                uint32_t least = ~0u;
+#pragma unroll
+                for (int c = 0; c < KC; ++c)
+#pragma unroll
+                    for (int j = 0; j < E; ++j) least = min(least, size_order(q[c][j]));
+                if (__any(least < size_order(TT::kLeast))) return false;
             }
 #pragma unroll
             for (int c = 0; c < KC; ++c)
@@ -566,7 +587,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_attend_mfma_kerne
                     }
                 }
             }
-            v4f sc = {0.0f, 0.0f, 0.0f, 0.0f};
+            v4f sc = {0.0f, 0.0f, 0.0f, 0.0f}, sc_low = sc;
 #pragma unroll
             for (int c = 0; c < KC; ++c) {
                 if constexpr (EXACT) {
@@ -576,11 +597,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_attend_mfma_kerne
                     for (int j = 0; j < E; ++j) sc = __builtin_amdgcn_mfma_f32_16x16x4f32(f[j], q[c][j], sc, 0, 0, 0);
                 } else {  // the small terms first
 #pragma unroll
-                    for (int t = TT::N - 1; t >= 0; --t) sc = TT::scores(kw[c], qt[t][c], sc);
+                    for (int t = TT::N - 1; t >= 0; --t) {
+                        v4f& to = APART && t ? sc_low : sc;
+                        to = TT::scores(kw[c], qt[t][c], to);
+                    }
                 }
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
+                if constexpr (APART) sc[i] = fmaf(sc_low[i], 1.0f / TT::kApart, sc[i]);
                 if constexpr (!EXACT && TT::kTop != 0.0f) sc[i] *= unscale;
                 sc[i] = vrow[i] != kBadRow ? sc[i] : -INFINITY;
             }
@@ -607,10 +632,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_attend_mfma_kerne
             }
             const float safe = m == -INFINITY ? 0.0f : m;
             float p[4];
+            uint32_t least = ~0u;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 p[i] = __builtin_amdgcn_exp2f(sc[i] - safe);
                 l += p[i];
+                least = min(least, size_order(p[i]));
+            }
+            if constexpr (APART) {
+                if (__any(least < size_order(TT::kLeast))) return false;
             }
             if constexpr (EXACT) {
 #pragma unroll
@@ -635,27 +665,47 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_attend_mfma_kerne
                         v[j] = u2{__builtin_amdgcn_perm(vw[1][c][j / 2], vw[0][c][j / 2], sel),
                                   __builtin_amdgcn_perm(vw[3][c][j / 2], vw[2][c][j / 2], sel)};
                     }
+                    if constexpr (APART) {
+                        // the later term's sums of a tile alone: held over all tiles they took as many registers as acc
 #pragma unroll
-                    for (int t = TT::N - 1; t >= 0; --t)  // independent products between those of one sum
+                        for (int j0 = 0; j0 < VE; j0 += 2) {
+                            v4f low[2];
 #pragma unroll
-                        for (int j = 0; j < VE; ++j) acc[c][j] = TT::output(u2{w0[t], w1[t]}, v[j], acc[c][j]);
+                            for (int j = 0; j < 2; ++j) low[j] = TT::output(u2{w0[1], w1[1]}, v[j0 + j], v4f{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) acc[c][j0 + j] = TT::output(u2{w0[0], w1[0]}, v[j0 + j], acc[c][j0 + j]);
+#pragma unroll
+                            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) acc[c][j0 + j][r] = fmaf(low[j][r], 1.0f / TT::kApart, acc[c][j0 + j][r]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int t = TT::N - 1; t >= 0; --t)  // independent products between those of one sum
+#pragma unroll
+                            for (int j = 0; j < VE; ++j) acc[c][j] = TT::output(u2{w0[t], w1[t]}, v[j], acc[c][j]);
+                    }
                 }
             }
         }
+        return true;
     };
     __syncthreads();
     if constexpr (!TT::kSplit) {
         run(std::true_type{});
     } else {
-        run(std::false_type{});
-        float bad = l * 0.0f;  // NaN where a sum is not finite
+        bool again = !run(std::false_type{});
+        if (!again) {
+            float bad = l * 0.0f;  // NaN where a sum is not finite
 #pragma unroll
-        for (int c = 0; c < VC; ++c)
+            for (int c = 0; c < VC; ++c)
 #pragma unroll
-            for (int j = 0; j < VE; ++j)
+                for (int j = 0; j < VE; ++j)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) bad += acc[c][j][r] * 0.0f;
-        if (__any(bad != bad)) run(std::true_type{});
+                    for (int r = 0; r < 4; ++r) bad += acc[c][j][r] * 0.0f;
+            again = __any(bad != bad);
+        }
+        if (again) run(std::true_type{});
     }
     l = fold_lanes<16, 64>(l, Sum());
     if (lane < 16) s_ml[wave][lane] = make_float2(m, l);

@@ -422,6 +422,70 @@ def test_small_and_large_values(ctx, dtype, unit, heads):
         assert np.all(np.abs(got[s] - out) <= tol + n * 2.0 ** -149), (s, float(np.abs(got[s] - out).max()))
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("heads,dim", [(1, 64), (5, 64), (3, 128), (17, 256)])
+def test_probabilities_far_below_the_greatest(ctx, dtype, heads, dim):
+    """One heavy key with small, subnormal or zero values beside keys that are up to 70 octaves lighter and have large
+    values: every probability keeps the bits that f32 gives it, whatever the others are.
+    A score is one product here, off by at most 5 u of itself (the scale folded into q, the product, the exponential's
+    argument), so a probability and the sum of them are off by 5 u S + 2^-22 and n + 64 roundings each."""
+    _say(f"light keys with large values, {dtype}, {heads} heads, {dim} wide")
+    rng = np.random.default_rng(16)
+    octaves = [4, 14, 15, 18, 24, 27, 28, 29, 30, 34, 38, 41, 48, 70]
+    n = 150
+    host = Host(rng, ctx, [n] * len(octaves), 16, 1, dim, dtype)
+    q = np.zeros((len(octaves), heads, dim), np.float32)
+    q[:, :, 0] = 1 + 0.01 * np.arange(heads)
+    for s, deep in enumerate(octaves):
+        heavy = int(rng.integers(n))
+        for j in range(n):
+            k, v = np.zeros((1, dim)), rng.standard_normal((1, dim)) * 2.0 ** 13
+            k[0, 0] = -deep * np.log(2) * rng.uniform(0.95, 1.0)
+            if j == heavy:
+                k[0, 0], v = 0.0, np.resize([2.0 ** -10, 0.0, 2.0 ** -24, 1.0], (1, dim))
+            host.put(s, j, k, v)
+    host.dk.copy_from(_bits(host.k, dtype))
+    host.dv.copy_from(_bits(host.v, dtype))
+    dout = ctx.empty((len(octaves), heads * dim), np.float32)
+    host.cache.attention(ctx.to_device(q.reshape(len(octaves), -1)), host.dt, host.dl, dout, scale=1.0)
+    got = dout.numpy().reshape(q.shape)
+    for s, deep in enumerate(octaves):
+        k, v = host.rows(s, np.arange(n))
+        for h in range(heads):
+            sc = k[:, 0, 0] * float(q[s, h, 0])
+            p = np.exp(sc - sc.max())
+            p /= p.sum()
+            tol = (p @ np.abs(v[:, 0])) * 2 * (5 * U * np.abs(sc).max() + 2.0 ** -22 + (n + 64) * U)
+            assert np.all(np.abs(got[s, h] - p @ v[:, 0]) <= tol), (deep, h, float((np.abs(got[s, h] - p @ v[:, 0]) / tol).max()))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("heads,dim", [(2, 128), (4, 64), (16, 128), (20, 256)])
+def test_query_rows_of_mixed_magnitude(ctx, dtype, heads, dim):
+    """A query row with one coordinate far above the others, where the keys are zero: the others keep their bits."""
+    _say(f"mixed query rows, {dtype}, {heads} heads, {dim} wide")
+    rng = np.random.default_rng(17)
+    far = [0, 12, 16, 20, 24, 27, 28, 29, 32, 36]  # octaves between the large coordinate and the others
+    n = 100
+    host = Host(rng, ctx, [n] * len(far), 32, 1, dim, dtype)
+    for s in range(len(far)):
+        for j in range(n):
+            k = rng.standard_normal((1, dim)) * 2.0 ** 12
+            k[0, 7] = 0.0
+            host.put(s, j, k, rng.standard_normal((1, dim)))
+    host.dk.copy_from(_bits(host.k, dtype))
+    host.dv.copy_from(_bits(host.v, dtype))
+    q = (rng.standard_normal((len(far), heads, dim)) * 2.0 ** -11).astype(np.float32)
+    for s, octaves in enumerate(far):
+        q[s, :, 7] = 2.0 ** (octaves - 11)
+    dout = ctx.empty((len(far), heads * dim), np.float32)
+    host.cache.attention(ctx.to_device(q.reshape(len(far), -1)), host.dt, host.dl, dout)
+    got = dout.numpy().reshape(q.shape)
+    for s, octaves in enumerate(far):
+        out, tol, _, _, _ = _attend(host, s, q[s], n, 0, 0, 1.0 / np.sqrt(np.float32(dim)))
+        assert np.all(np.abs(got[s] - out) <= tol), (octaves, float((np.abs(got[s] - out) / tol).max()))
+
+
 def test_far_offsets(ctx):
     """Pages past 2^32 bytes and 2^31 values of a pool."""
     _say("far offsets")
