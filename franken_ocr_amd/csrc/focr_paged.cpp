@@ -501,6 +501,8 @@ int32_t focr_hip_beam_reorder(focr_hip_ctx* ctx, size_t groups, size_t beams, co
                 ring_rows = std::max(ring_rows, c->ring_len[s]);
             }
         }
+        // a graph's replays find the rings further on than the capture did: whole windows follow
+        if (n_rings && ctx->captures()) ring_rows = kRingWindow;
         if (check) {
             Check k{ctx};
             if ((st = k.begin(who))) return st;

@@ -537,7 +537,9 @@ int32_t focr_hip_beam_select(focr_hip_ctx* ctx, const float* logits, size_t ld, 
  *    same length throughout a group; the entry of that page and those after it
  *    stay the slot's own, and the page takes the parent's rows;
  *  - its ring's rows in each of `rings` (streams g * beams + b, with the same
- *    prompt and the same cursors throughout a group, E_STATE otherwise).
+ *    prompt and the same cursors throughout a group, E_STATE otherwise; a
+ *    captured call moves whole rings, so its replays may find them at other
+ *    cursors, whose agreement is the caller's to keep).
  * So the beams of a group may share the pages they have filled and must not
  * share the one in progress. A parent that is not below beams is taken as the
  * slot itself, a group whose lengths differ keeps its tables and pages;

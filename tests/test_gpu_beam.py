@@ -485,6 +485,57 @@ def test_beam_search_over_the_decoder(ctx, model):  # noqa: F811
     assert np.all(np.abs(got - want) <= steps * (2.0 ** -24 * np.abs(want) + 1e-9)), (got, want)
 
 
+@pytest.mark.parametrize("before", [0, 3])
+def test_captured_reorder_of_rings_that_grow(ctx, before):
+    """Rings reordered by a graph that was captured when they held `before` rows, replayed after eager steps: every
+    row that they hold by then follows its parent, as by an eager call."""
+    _say(f"captured, rings of {before} rows")
+    from franken_ocr_amd.device import Context
+    from franken_ocr_amd.engine import RingCache, beam_reorder
+
+    c = Context(0)
+    rng = np.random.default_rng(43)
+    groups, beams, D = 2, 3, 1280
+    rows = groups * beams
+    rings = [RingCache(rows, 8, ctx=c) for _ in "ab"]  # by the graph, by eager calls
+    for s in range(rows):
+        k = c.to_device(rng.standard_normal((10, 4, 128)).astype(np.float32))
+        for ring in rings:
+            ring.record_prefill(s, k, k, 4)
+    p, out = c.empty((rows,), np.uint32), c.empty((rows, D), np.float32)
+
+    def steps(n):
+        for _ in range(n):
+            q, k, v = (c.to_device(rng.standard_normal((rows, D)).astype(np.float32)) for _ in "qkv")
+            for ring in rings:
+                ring.step(q, k, v, out)
+            c.synchronize()  # before the rows go
+
+    def held(ring):
+        got = []
+        for s in range(rows):
+            at = ring.regions(s)
+            for name in ("ring_k", "ring_v"):
+                x = np.empty((10, 128, 128), np.float32)
+                _abi.call("focr_hip_d2h", c.handle, x.ctypes.data, at[name], x.nbytes)
+                got.append(x)
+        return np.stack(got)
+
+    steps(before)
+    replay = _capture(c, lambda: beam_reorder(p, beams, rings=[rings[0]]))
+    count = before
+    for more in (2, 5, 60, 100):  # the last past the rings' end
+        steps(more)
+        count = min(128, count + more)
+        parents = rng.integers(0, beams, rows).astype(np.uint32)
+        p.copy_from(parents)
+        assert replay() == 0
+        c.synchronize()
+        beam_reorder(p, beams, rings=[rings[1]])
+        a, b = held(rings[0])[:, :, :count], held(rings[1])[:, :, :count]
+        assert np.array_equal(a, b), more
+
+
 def test_captured_beam_step_replays(ctx):
     """Selection and reordering in one graph, replayed on changing logits, against the same calls made eagerly."""
     _say("captured")
