@@ -123,6 +123,8 @@ _SIGS: dict[str, list] = {
     "focr_hip_beam_select": [_P, _P, _SZ, _SZ, _SZ, _SZ, _P, _P, C.c_uint32, _P, _SZ, _P, _SZ, _SZ, _P, _SZ, _P, _P, _P,
                              _P, _I32],
     "focr_hip_beam_reorder": [_P, _SZ, _SZ, _P, _P, _P, _SZ, _P, _I32, _P, _SZ, _P, _SZ, _P, _P, _SZ, _I32],
+    "focr_hip_beam_reorder_weighted": [_P, _SZ, _SZ, _P, _P, _P, _SZ, _P, _I32, _P, _SZ, _P, _SZ, _P, _P, _SZ, _P, _SZ,
+                                       _I32],
     "focr_hip_focrq_open": [C.c_char_p, _P],
     "focr_hip_focrq_from_bytes": [_P, _SZ, _P],
     "focr_hip_focrq_close": [_P],

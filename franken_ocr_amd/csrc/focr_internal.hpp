@@ -825,6 +825,9 @@ struct BeamReorder {
 hipError_t launch_beam_reorder(hipStream_t s, const BeamReorder& a, const focr_hip_paged* const* caches,
                                size_t n_caches, const focr_hip_rswa* const* rings, size_t n_rings,
                                uint32_t ring_rows);
+// weights[i] (nullable) of caches[i], [rows][its n_kv_heads][ldw]
+hipError_t launch_beam_weights(hipStream_t s, const BeamReorder& a, const focr_hip_paged* const* caches,
+                               float* const* weights, size_t n, size_t ldw);
 hipError_t launch_beam_check(hipStream_t s, const BeamReorder& a, unsigned long long* err);
 
 }  // namespace focr

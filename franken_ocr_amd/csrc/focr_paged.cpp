@@ -446,6 +446,16 @@ int32_t focr_hip_beam_reorder(focr_hip_ctx* ctx, size_t groups, size_t beams, co
                               int32_t advance, focr_hip_paged* const* caches, size_t n_caches, uint32_t* tables,
                               size_t max_pages, const uint32_t* lens, focr_hip_rswa* const* rings, size_t n_rings,
                               int32_t check) {
+    return focr_hip_beam_reorder_weighted(ctx, groups, beams, parents, tokens, history, history_cap, history_len, advance,
+                                          caches, n_caches, tables, max_pages, lens, nullptr, 0, rings, n_rings, check);
+}
+
+int32_t focr_hip_beam_reorder_weighted(focr_hip_ctx* ctx, size_t groups, size_t beams, const uint32_t* parents,
+                                       const uint32_t* tokens, uint32_t* history, size_t history_cap,
+                                       uint32_t* history_len, int32_t advance, focr_hip_paged* const* caches,
+                                       size_t n_caches, uint32_t* tables, size_t max_pages, const uint32_t* lens,
+                                       float* const* weights, size_t ldw, focr_hip_rswa* const* rings, size_t n_rings,
+                                       int32_t check) {
     return entry(ctx, [&]() -> int32_t {
         const char* who = "beam_reorder";
         if (groups == 0) return FOCR_HIP_OK;
@@ -474,6 +484,12 @@ int32_t focr_hip_beam_reorder(focr_hip_ctx* ctx, size_t groups, size_t beams, co
                     return fail(FOCR_HIP_E_ARG, fmt("beam_reorder: caches %zu and %zu are the same", j, i));
             if (caches[i]->page_shift != caches[0]->page_shift)
                 return fail(FOCR_HIP_E_SHAPE, "beam_reorder: caches of different page sizes share no tables");
+            if (!weights || !weights[i]) continue;
+            if (ldw == 0 || ldw > kMaxLen)
+                return fail(FOCR_HIP_E_SHAPE, fmt("beam_reorder: ldw %zu is outside 1 .. %zu", ldw, kMaxLen));
+            for (size_t j = 0; j < i; ++j)
+                if (weights[i] == weights[j])
+                    return fail(FOCR_HIP_E_ARG, fmt("beam_reorder: the weights of caches %zu and %zu are the same", j, i));
         }
         if (n_caches) {
             PagedTables t;
@@ -516,6 +532,8 @@ int32_t focr_hip_beam_reorder(focr_hip_ctx* ctx, size_t groups, size_t beams, co
             if (n_caches && (st = k.end(who, "row"))) return st;
         }
         ProfScope ps(ctx, "beam_reorder");
+        if (weights)
+            FOCR_HIP_TRY(launch_beam_weights(ctx->stream, a, caches, weights, n_caches, ldw), "beam weights launch");
         FOCR_HIP_TRY(launch_beam_reorder(ctx->stream, a, caches, n_caches, rings, n_rings, ring_rows), "beam reorder launch");
         return FOCR_HIP_OK;
     });

@@ -531,6 +531,35 @@ __global__ __launch_bounds__(256) void beam_reorder_kernel(BeamReorder a, Stores
     });
 }
 
+// The weights that attention gathered for the keys of each slot's cache, of up
+// to kStores caches: [rows][heads][ld] each.
+struct Gathered {
+    float* w[kStores];
+    uint32_t heads[kStores];
+    int n;
+    size_t ld;
+    uint32_t pieces;  // blocks to a head's row
+};
+
+// Grid (head x piece, group, cache): a thread a key of every slot.
+template <int WB>
+__global__ __launch_bounds__(256) void beam_weights_kernel(BeamReorder a, Gathered w) {
+    __shared__ uint32_t s_parent[WB];
+    const int grp = blockIdx.y;
+    const uint32_t head = blockIdx.x / w.pieces;
+    const size_t first = (blockIdx.x - head * w.pieces) * 256u;
+    const size_t heads = w.heads[blockIdx.z];
+    if (head >= heads) return;
+    const Group g = group_of(a, grp);
+    const size_t n = min(static_cast<size_t>(g.len), w.ld);
+    if (!g.ok || first >= n) return;
+    if (threadIdx.x < a.beams) s_parent[threadIdx.x] = parent_of(a, grp, threadIdx.x);
+    __syncthreads();
+    uint32_t* base = reinterpret_cast<uint32_t*>(w.w[blockIdx.z]) + (static_cast<size_t>(grp) * a.beams * heads + head) * w.ld;
+    permute_columns<WB, uint32_t>(s_parent, a.beams, n, first + threadIdx.x, 256 * w.pieces,
+                                  [&](uint32_t b, size_t i) { return base + b * heads * w.ld + i; });
+}
+
 __global__ void beam_check_kernel(BeamReorder a, unsigned long long* err) {
     const int grp = blockIdx.x;
     const size_t row0 = static_cast<size_t>(grp) * a.beams;
@@ -625,6 +654,36 @@ hipError_t launch_beam_reorder(hipStream_t s, const BeamReorder& a, const focr_h
         if (e != hipSuccess) return e;
         now.history = nullptr;  // once; and the tables too, whose entries of the pages in progress stay as they are
         now.permute = 0;
+    }
+    return hipSuccess;
+}
+
+hipError_t launch_beam_weights(hipStream_t s, const BeamReorder& a, const focr_hip_paged* const* caches,
+                               float* const* weights, size_t n, size_t ldw) {
+    Gathered w{};
+    uint32_t heads = 0;
+    w.ld = ldw;
+    w.pieces = static_cast<uint32_t>(std::min<size_t>((ldw + 255) / 256, 256));
+    for (size_t i = 0; i < n; ++i) {
+        if (weights[i]) {
+            w.w[w.n] = weights[i];
+            w.heads[w.n++] = static_cast<uint32_t>(caches[i]->n_kv_heads);
+            heads = std::max(heads, static_cast<uint32_t>(caches[i]->n_kv_heads));
+        }
+        if (w.n == 0 || (w.n < kStores && i + 1 < n)) continue;
+        const dim3 grid(heads * w.pieces, a.groups, w.n);
+        if (a.beams <= 4)
+            FOCR_LAUNCH(beam_weights_kernel<4>, grid, dim3(256), 0, s, a, w);
+        else if (a.beams <= 8)
+            FOCR_LAUNCH(beam_weights_kernel<8>, grid, dim3(256), 0, s, a, w);
+        else if (a.beams <= 16)
+            FOCR_LAUNCH(beam_weights_kernel<16>, grid, dim3(256), 0, s, a, w);
+        else
+            FOCR_LAUNCH(beam_weights_kernel<32>, grid, dim3(256), 0, s, a, w);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        w.n = 0;
+        heads = 0;
     }
     return hipSuccess;
 }

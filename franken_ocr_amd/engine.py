@@ -545,11 +545,14 @@ def beam_select(logits: DeviceArray, scores: DeviceArray, beams: int, parents: D
 def beam_reorder(parents: DeviceArray, beams: int, tokens: DeviceArray | None = None,
                  history: DeviceArray | None = None, history_len: DeviceArray | None = None, advance: bool = False,
                  caches: list[PagedCache] = (), tables: DeviceArray | None = None, lens: DeviceArray | None = None,
-                 rings: list[RingCache] = (), check: bool = False) -> None:
+                 rings: list[RingCache] = (), check: bool = False,
+                 weights: list[DeviceArray | None] | None = None) -> None:
     """The states of the chosen beams put where their slots are, in place: slot
     b of each group takes slot parents[b]'s history (then tokens[b] behind it),
     the entries of its page table up to the page in progress and that page's
-    rows in every cache (one per layer, sharing the tables), and its rings."""
+    rows in every cache (one per layer, sharing the tables), what each cache's
+    attention has gathered in its weights [rows, n_kv_heads, slots] (one array,
+    or None, per cache; all of one width), and its rings."""
     rows, beams = parents.shape[0], int(beams)
     if beams <= 0 or rows % beams:
         raise _abi.ContractViolation(_abi.E_SHAPE, f"beam_reorder: {rows} rows are no groups of {beams}")
@@ -563,9 +566,18 @@ def beam_reorder(parents: DeviceArray, beams: int, tokens: DeviceArray | None = 
     fits("beam_reorder", "tables", tables, rows, wide)
     paged = (C.c_void_p * len(caches))(*[c._h.value for c in caches]) if caches else None
     ring = (C.c_void_p * len(rings))(*[c._h.value for c in rings]) if rings else None
-    _abi.call("focr_hip_beam_reorder", parents.ctx.handle, rows // beams, beams, _p(parents), _p(tokens), _p(history),
-              cap, _p(history_len), 1 if advance else 0, paged, len(caches), _p(tables), wide, _p(lens), ring,
-              len(rings), 1 if check else 0)
+    gathered, ldw = None, 0
+    if weights is not None:
+        if len(weights) != len(caches):
+            raise _abi.ContractViolation(_abi.E_SHAPE, f"beam_reorder: {len(weights)} weights for {len(caches)} caches")
+        widths = {c._weights("beam_reorder", w, rows) for c, w in zip(caches, weights) if w is not None}
+        if len(widths) > 1:
+            raise _abi.ContractViolation(_abi.E_SHAPE, f"beam_reorder: weights of widths {sorted(widths)}")
+        if widths:
+            gathered, ldw = (C.c_void_p * len(weights))(*[None if w is None else w.ptr for w in weights]), widths.pop()
+    _abi.call("focr_hip_beam_reorder_weighted", parents.ctx.handle, rows // beams, beams, _p(parents), _p(tokens),
+              _p(history), cap, _p(history_len), 1 if advance else 0, paged, len(caches), _p(tables), wide, _p(lens),
+              gathered, ldw, ring, len(rings), 1 if check else 0)
 
 
 def prefill_chunk_bounds(seq: int, chunk: int) -> list:

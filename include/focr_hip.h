@@ -550,6 +550,18 @@ int32_t focr_hip_beam_reorder(focr_hip_ctx* ctx, size_t groups, size_t beams, co
                               size_t n_caches, uint32_t* tables, size_t max_pages, const uint32_t* lens,
                               focr_hip_rswa* const* rings, size_t n_rings, int32_t check);
 
+/* The same where the caches' attention gathers weights: weights[i] (nullable) is
+ * what caches[i] has gathered, [groups * beams][its n_kv_heads][ldw], and slot b
+ * takes the first min(lens[row], ldw) of slot parents[b]'s, as it takes its
+ * keys; without them an eviction would cut a slot's new keys by the weights of
+ * its old ones. A group whose tables stay keeps its weights. */
+int32_t focr_hip_beam_reorder_weighted(focr_hip_ctx* ctx, size_t groups, size_t beams, const uint32_t* parents,
+                                       const uint32_t* tokens, uint32_t* history, size_t history_cap,
+                                       uint32_t* history_len, int32_t advance, focr_hip_paged* const* caches,
+                                       size_t n_caches, uint32_t* tables, size_t max_pages, const uint32_t* lens,
+                                       float* const* weights, size_t ldw, focr_hip_rswa* const* rings, size_t n_rings,
+                                       int32_t check);
+
 /* nn.rs:240-253 rms_norm over rows x [rows, n] f32 -> y (device pointers; w
  * [n] device, nullable): y = (x * rstd) * w, rstd = 1 / sqrt(mean(x^2) + eps)
  * with the sum of squares in f64. n <= 4096. The final norm before the LM

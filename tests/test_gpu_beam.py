@@ -360,6 +360,124 @@ def test_reorder_without_check_leaves_what_is_no_group(ctx):
     host.same_pools()
 
 
+@pytest.mark.parametrize("beams,groups,kv,ldw,length,layers", [(2, 3, 3, 77, 40, 2), (5, 2, 1, 1000, 999, 35), (8, 1, 10, 64, 1, 1),
+                                                               (13, 2, 2, 4099, 4098, 2), (32, 1, 1, 300, 257, 1)])
+def test_reorder_moves_gathered_weights(ctx, beams, groups, kv, ldw, length, layers):
+    """Every cache's gathered weights up to the length follow the parents, exactly; what lies behind it, a group that
+    is none, a cache without weights: as they were."""
+    _say(f"reorder weights {groups} x {beams}, {layers} layers")
+    from franken_ocr_amd.engine import PagedCache, beam_reorder
+
+    rng = np.random.default_rng(beams)
+    rows, page, wide = groups * beams, 32, -(-(length + 40) // 32)
+    lens = np.repeat([length if g != 1 else length + 7 for g in range(groups)], beams).astype(np.uint32)  # one past ldw
+    if groups == 3:
+        lens[-1] += 1  # no group: its lengths differ
+    caches = [PagedCache(rows * wide, page, kv + i % 2, 64, "bf16", ctx=ctx) for i in range(layers)]
+    tables = np.arange(rows * wide, dtype=np.uint32).reshape(rows, wide)
+    w = [None if i == 1 else rng.random((rows, kv + i % 2, ldw)).astype(np.float32) for i in range(layers)]
+    dw = [x if x is None else ctx.to_device(x) for x in w]
+    parents = rng.integers(0, beams, rows).astype(np.uint32)
+    dt = ctx.to_device(tables)
+    beam_reorder(ctx.to_device(parents), beams, caches=caches, tables=dt, lens=ctx.to_device(lens), weights=dw)
+    same = [len(set(lens[g * beams:(g + 1) * beams].tolist())) == 1 for g in range(groups)]
+    src = np.array([r // beams * beams + parents[r] if same[r // beams] else r for r in range(rows)])
+    for x, d in zip(w, dw):
+        if x is not None:
+            want = x.copy()
+            for r in range(rows):
+                want[r, :, :lens[r]] = x[src[r], :, :lens[r]]
+            assert np.array_equal(d.numpy(), want)
+    assert np.array_equal(dt.numpy()[:, :1], tables[src, :1] if length >= page else tables[:, :1])
+
+
+def test_search_gathers_and_evicts_by_its_own_beams(ctx):
+    """Steps that gather weights, reordered by drawn parents, then the eviction: each slot's weights are those of its
+    ancestors' probabilities, kept apart on the host in 64 bits, and what it keeps are its own keys."""
+    _say("weights of beams")
+    from franken_ocr_amd.engine import PagedCache, beam_reorder
+    from test_gpu_paged import _attend, _stay
+
+    rng = np.random.default_rng(47)
+    groups, beams, kv, heads, dim, page, steps, wide = 2, 3, 2, 6, 64, 8, 25, 8
+    rows, prompts = groups * beams, [19, 8]
+    cache = PagedCache(rows * (wide + 2), page, kv, dim, "f32", ctx=ctx)
+    order = rng.permutation(rows * (wide + 2)).astype(np.uint32)
+    tables, dst = order[: rows * wide].reshape(rows, wide).copy(), order[rows * wide:].reshape(rows, 2)
+
+    class Beam:
+        def __init__(self, k, v):
+            self.kv, self.k, self.v = kv, k, v
+            self.w, self.tol = np.zeros((kv, wide * page)), np.zeros((kv, wide * page))
+
+        def rows(self, s, keys):
+            return self.k[keys].astype(np.float64), self.v[keys].astype(np.float64)
+
+        def after(self, k, v):
+            b = Beam(np.concatenate([self.k, k[None]]), np.concatenate([self.v, v[None]]))
+            b.w, b.tol = self.w.copy(), self.tol.copy()
+            return b
+
+    host = []
+    for g in range(groups):
+        k, v = (rng.standard_normal((prompts[g], kv, dim)).astype(np.float32) for _ in "kv")
+        for b in range(beams):
+            host.append(Beam(k, v))
+    dt = ctx.to_device(tables)
+    for r in range(rows):
+        n = prompts[r // beams]
+        flat = [ctx.to_device(x.reshape(n, -1)) for x in (host[r].k, host[r].v)]
+        cache.write(*flat, ctx.to_device(np.arange(n, dtype=np.uint32)), dt, seq=ctx.to_device(np.full(n, r, np.uint32)), check=True)
+    lens = ctx.to_device(np.repeat(prompts, beams).astype(np.uint32))
+    dw, out = ctx.to_device(np.zeros((rows, kv, wide * page), np.float32)), ctx.empty((rows, heads * dim), np.float32)
+    scale = 1.0 / np.sqrt(np.float32(dim))
+    for i in range(steps):
+        q = rng.standard_normal((rows, heads, dim)).astype(np.float32) * 2
+        k, v = (rng.standard_normal((rows, kv, dim)).astype(np.float32) for _ in "kv")
+        cache.step(ctx.to_device(q.reshape(rows, -1)), ctx.to_device(k.reshape(rows, -1)), ctx.to_device(v.reshape(rows, -1)),
+                   dt, lens, out, weights=dw, advance=True, check=True)
+        for r in range(rows):
+            host[r] = host[r].after(k[r], v[r])
+            _, _, keys, w, wt = _attend(host[r], 0, q[r], len(host[r].k), 0, 0, scale)
+            host[r].w[:, keys] += w
+            host[r].tol[:, keys] += wt + 2.0 ** -24 * (1 + host[r].w[:, keys])
+        parents = rng.integers(0, beams, rows).astype(np.uint32)
+        beam_reorder(ctx.to_device(parents), beams, caches=[cache], tables=dt, lens=lens, weights=[dw], check=True)
+        host = [host[r // beams * beams + parents[r]] for r in range(rows)]
+        got = dw.numpy()
+        for r in range(rows):
+            assert np.all(np.abs(got[r] - host[r].w) <= host[r].tol), (i, r)
+    budget, dst_w = 2 * page, ctx.empty((rows, kv, 2 * page), np.float32)
+    kept = ctx.empty((rows, kv, budget), np.uint32)
+    cache.evict(dt, lens, dw, budget, ctx.to_device(dst), lens, dst_w, sinks=1, recent=3, kept=kept, check=True)
+    pools = []
+    for at in cache.regions().values():
+        x = np.empty((rows * (wide + 2), kv, page, dim), np.float32)
+        _abi.call("focr_hip_d2h", ctx.handle, x.ctypes.data, at, x.nbytes)
+        pools.append(x)
+    slots = np.arange(budget)
+    for r in range(rows):
+        for h in range(kv):
+            stay = _stay(got[r, h], len(host[r].k), budget, 1, 3)
+            assert np.array_equal(kept.numpy()[r, h], stay)
+            for x, rows_of in zip(pools, (host[r].k, host[r].v)):
+                assert np.array_equal(x[dst[r, slots // page], h, slots % page], rows_of[stay, h])
+
+
+def test_reorder_refuses_weights_that_do_not_fit(ctx):
+    _say("refusals of weights")
+    from franken_ocr_amd.engine import PagedCache, beam_reorder
+
+    caches = [PagedCache(4, 16, 1, 64, ctx=ctx) for _ in "ab"]
+    u, w = (lambda *s: ctx.to_device(np.zeros(s, np.uint32))), (lambda *s: ctx.to_device(np.zeros(s, np.float32)))
+    one = w(2, 1, 32)
+    for weights, text in (([one], "1 weights for 2 caches"), ([one, w(2, 2, 32)], "weights of shape"),
+                          ([w(2, 1, 16), one], "widths"), ([one, one], "are the same"), ([one, w(1, 1, 32)], "weights of shape"),
+                          ([w(2, 1, 0), w(2, 1, 0)], "ldw 0")):
+        with pytest.raises(_abi.FocrHipError, match=text):
+            beam_reorder(u(2), 2, caches=caches, tables=u(2, 2), lens=u(2), weights=weights)
+
+
 def test_beam_search_over_pages_and_rings(ctx):
     """Eight steps of search with a little model (one attention over what was read): the paged cache whose beams
     share the prompt's pages, and the ring caches, against every beam's keys kept apart on the host in 64 bits."""
