@@ -60,6 +60,46 @@ def test_step_refuses_arrays_that_do_not_fit(change, text):
                       weights=a.get("weights"), n_heads=4)
 
 
+@pytest.mark.parametrize("shapes,n_heads,want", [
+    # q, k, v, out of four rows; what the call passes on: heads, ldq, ldkv, ldo
+    (((4, 256), (4, 128), (4, 128), (4, 256)), None, (4, 256, 128, 256)),
+    (((4, 512), (4, 200), (4, 200), (4, 300)), 4, (4, 512, 200, 300)),      # wider rows: the arrays' widths
+    (((4, 4, 64), (4, 2, 64), (4, 2, 64), (4, 4, 64)), None, (4, 256, 128, 256)),
+    (((6, 260), (9, 128), (5, 128), (4, 256)), 4, (4, 260, 128, 256)),      # more rows than are read
+    (((1024,), (8, 64), (512,), (2, 512)), 4, (4, 256, 128, 256)),          # flat, or in rows of their own
+])
+def test_row_strides_are_the_arrays_widths(monkeypatch, shapes, n_heads, want):
+    from franken_ocr_amd import _abi
+
+    seen = {}
+    monkeypatch.setattr(_abi, "call", lambda name, *a: seen.update({name: a}))
+    q, k, v, out = (_array(s) for s in shapes)
+    tables, lens = _array((4, 2), np.uint32), _array((4,), np.uint32)
+    _cache().step(q, k, v, tables, lens, out, n_heads=n_heads)
+    a = seen["focr_hip_paged_step"]
+    assert (a[4], a[3], a[7], a[17]) == want
+    _cache().attention(q, tables, lens, out, n_heads=n_heads)
+    a = seen["focr_hip_paged_attention"]
+    assert (a[4], a[3], a[14]) == (want[0], want[1], want[3])
+    _cache().write(k, v, lens, tables)
+    assert seen["focr_hip_paged_write"][4] == want[2]
+    _cache().step(q, k, v, tables, lens, out, n_heads=2, ldq=129, ldkv=128, ldo=130)  # given ones come first
+    a = seen["focr_hip_paged_step"]
+    assert (a[4], a[3], a[7], a[17]) == (2, 129, 128, 130)
+
+
+@pytest.mark.parametrize("shapes,text", [
+    (((4, 250), (4, 128), (4, 128), (4, 256)), "no whole heads"),
+    (((4, 256), (4, 128), (4, 130), (4, 256)), "k_steps rows of 128 and v_steps rows of 130"),
+])
+def test_step_refuses_rows_of_no_one_width(shapes, text):
+    from franken_ocr_amd import _abi
+
+    q, k, v, out = (_array(s) for s in shapes)
+    with pytest.raises(_abi.ContractViolation, match=text):
+        _cache().step(q, k, v, _array((4, 2), np.uint32), _array((4,), np.uint32), out)
+
+
 def test_beam_calls_refuse_rows_that_are_no_groups():
     from franken_ocr_amd import _abi, engine
 
