@@ -58,6 +58,8 @@ enum ScratchSlot : int {
     kScrPaged,  // paged attention: split partials, scores
     kScrEvict,  // eviction: selection tables, kept slots
     kScrBeam,   // beam selection: per-chunk candidates and sums
+    kScrBeamBan,   // beam selection's ban bitmaps and flags: not the sampler's, which
+    kScrBeamFlag,  // captured calls hold and a wider selection would outgrow
     kScrCheck,  // checks of paged / beam arguments: the first fault found
     kScrCount
 };

@@ -416,8 +416,8 @@ int32_t focr_hip_beam_select(focr_hip_ctx* ctx, const float* logits, size_t ld, 
             p.n_white = static_cast<int>(n_whitelist);
             p.vocab = a.vocab;
             p.ban_words = static_cast<int>(words);
-            p.ban_bits = static_cast<uint32_t*>(ctx->scratch_get_capturable(kScrBan, rows * words * sizeof(uint32_t), who));
-            p.err = static_cast<int*>(ctx->scratch_get_capturable(kScrFlag, rows * sizeof(int), who));
+            p.ban_bits = static_cast<uint32_t*>(ctx->scratch_get_capturable(kScrBeamBan, rows * words * sizeof(uint32_t), who));
+            p.err = static_cast<int*>(ctx->scratch_get_capturable(kScrBeamFlag, rows * sizeof(int), who));
             if (!p.ban_bits || !p.err) return no_scratch(ctx);
             if (check && ctx->captures())
                 return fail(FOCR_HIP_E_STATE, "beam_select: check = 1 waits for the stream and cannot be captured");

@@ -654,6 +654,43 @@ def test_captured_reorder_of_rings_that_grow(ctx, before):
         assert np.array_equal(a, b), more
 
 
+def test_selection_leaves_a_captured_samplers_scratch(ctx):
+    """A captured sampler call, then wider selections with a long ban: the graph's bitmaps and flags stay its own."""
+    _say("captured sampler beside selections")
+    from franken_ocr_amd.device import Context
+    from franken_ocr_amd.engine import beam_select, sample_rows
+
+    c = Context(0)
+    rng = np.random.default_rng(44)
+    vocab, cap = 3000, 300
+    text = np.resize(np.arange(2, 42), cap).astype(np.uint32)  # after 40 tokens every one of them ends a 2-gram again
+    logits = rng.standard_normal((2, vocab)).astype(np.float32)
+    logits[0, 12] = logits[1, 22] = 40.0  # what came after the last token 40 tokens ago, and what has not come yet
+    x, h, n = c.to_device(logits), c.to_device(np.stack([text, text])), c.to_device(np.array([90, 20], np.uint32))
+    tok = c.empty((2,), np.uint32)
+
+    def sample():
+        sample_rows(x, tok, h, n, 2, 0)
+
+    sample()
+    want = tok.numpy()
+    assert want[0] != 12 and want[1] == 22
+    replay = _capture(c, sample)
+    for rows, wide in ((8, 129280), (2000, 500)):
+        p, t, s = c.empty((rows,), np.uint32), c.empty((rows,), np.uint32), c.to_device(np.zeros(rows, np.float32))
+        beam_select(c.to_device(rng.standard_normal((rows, wide)).astype(np.float32)), s, 4, p, t, s,
+                    history=c.to_device(np.zeros((rows, cap), np.uint32)), history_len=c.to_device(np.full(rows, cap, np.uint32)),
+                    ngram_size=2, window=0)
+        held = [c.empty((1 << 16,), np.uint8) for _ in range(8)]  # takes what was freed, if anything was
+        for a in held:
+            a.copy_from(np.full(1 << 16, 255, np.uint8))
+        tok.copy_from(np.zeros(2, np.uint32))
+        assert replay() == 0
+        c.synchronize()
+        assert np.array_equal(tok.numpy(), want)
+        assert all(np.all(a.numpy() == 255) for a in held)
+
+
 def test_captured_beam_step_replays(ctx):
     """Selection and reordering in one graph, replayed on changing logits, against the same calls made eagerly."""
     _say("captured")
