@@ -110,13 +110,13 @@ struct Check {
     }
 };
 
-// The attention's workspace in one scratch slot.
-int32_t carve(focr_hip_ctx* ctx, const char* who, const focr_hip_paged* c, PagedAttend* a, bool scores) {
+// The attention's workspace in one scratch slot; seen_most: keys that a row sees at most.
+int32_t carve(focr_hip_ctx* ctx, const char* who, const focr_hip_paged* c, PagedAttend* a, bool scores, size_t seen_most) {
     const size_t n = a->t.n_seqs, heads = c->n_kv_heads * a->group, parts = n * heads * a->nsplit;
     const size_t seen = (n * sizeof(uint4) + 255) & ~size_t(255);
     const size_t acc = (parts * c->head_dim * sizeof(float) + 255) & ~size_t(255);
     const size_t ml = (parts * sizeof(float2) + 255) & ~size_t(255);
-    a->score_ld = scores ? a->t.max_len : 0;
+    a->score_ld = scores ? seen_most : 0;
     char* p = static_cast<char*>(
         ctx->scratch_get_capturable(kScrPaged, seen + acc + ml + n * heads * a->score_ld * sizeof(float), who));
     if (!p) return no_scratch(ctx);
@@ -174,7 +174,7 @@ int32_t attend(focr_hip_ctx* ctx, const char* who, const focr_hip_paged* c, cons
         FOCR_HIP_TRY(launch_paged_check(ctx->stream, c, a.t, step ? 1 : 0, prefix, a.window, k.err), "check launch");
         if ((st = k.end(who, "sequence"))) return st;
     }
-    if ((st = carve(ctx, who, c, &a, weights != nullptr))) return st;
+    if ((st = carve(ctx, who, c, &a, weights != nullptr, seen))) return st;
     FOCR_HIP_TRY(launch_paged_attend(ctx->stream, c, a, ctx), "paged attention launch");
     return FOCR_HIP_OK;
 }

@@ -1306,7 +1306,7 @@ hipError_t launch_paged_attend(hipStream_t s, const focr_hip_paged* c, const Pag
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     ProfScope ps(ctx, "paged_join");
-    const uint32_t chunks = a.weights ? (a.t.max_len + kWeightKeys - 1) / kWeightKeys : 0;
+    const uint32_t chunks = a.weights ? static_cast<uint32_t>((a.score_ld + kWeightKeys - 1) / kWeightKeys) : 0;
     const dim3 grid(kv * (a.group + chunks), a.t.n_seqs);
     // 1024 threads where a row has many splits to join (64 rows of 256 splits: 10 -> 7.5 us)
     const bool many = a.nsplit > 64;

@@ -486,6 +486,31 @@ def test_query_rows_of_mixed_magnitude(ctx, dtype, heads, dim):
         assert np.all(np.abs(got[s] - out) <= tol), (octaves, float((np.abs(got[s] - out) / tol).max()))
 
 
+def test_scores_of_a_window_take_the_windows_room(ctx):
+    """Weights under a window alone: scratch for the keys that it shows, whatever the tables hold, and the same results."""
+    _say("scores of a window")
+    from franken_ocr_amd.device import Context
+
+    c = Context(0)
+    rng = np.random.default_rng(18)
+    window, heads, dim = 100, 16, 64
+    host = Host(rng, c, [300, 100, 99, 0, NONE, 101, 1], 16, 2, dim, "bf16", wide=4096)  # 65536 slots
+    n = len(host.lens)
+    q = rng.standard_normal((n, heads, dim)).astype(np.float32)
+    dout, dw = c.empty((n, heads * dim), np.float32), c.to_device(np.zeros((n, 2, 65536), np.float32))
+    host.cache.attention(c.to_device(q.reshape(n, -1)), host.dt, host.dl, dout, window=window, weights=dw, check=True)
+    assert c.scratch_bytes() < 2 << 20  # 112 rows of scores over all slots take 29 MB, of two splits of 64 keys 0.1
+    got, gw = dout.numpy().reshape(n, heads, dim), dw.numpy()
+    for s, x in enumerate(host.lens):
+        if x == NONE:
+            continue
+        out, tol, keys, w, wt = _attend(host, s, q[s], x, 0, window, 1.0 / np.sqrt(np.float32(dim)))
+        assert np.all(np.abs(got[s] - out) <= tol), s
+        want, bound = np.zeros((2, 65536)), np.zeros((2, 65536))
+        want[:, keys], bound[:, keys] = w, wt + U * (1 + w)
+        assert np.all(np.abs(gw[s] - want) <= bound), s
+
+
 def test_far_offsets(ctx):
     """Pages past 2^32 bytes and 2^31 values of a pool."""
     _say("far offsets")
