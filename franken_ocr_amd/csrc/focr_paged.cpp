@@ -48,6 +48,17 @@ constexpr size_t kI32Max = static_cast<size_t>(std::numeric_limits<int32_t>::max
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+bool overlap(const void* a, const void* b, size_t a_bytes, size_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y ? y - x < a_bytes : x - y < b_bytes;
+}
+
+// Whether two caches' pools have memory in common.
+bool overlap(const focr_hip_paged* a, const focr_hip_paged* b) {
+    const size_t na = a->n_pages * a->page_bytes(), nb = b->n_pages * b->page_bytes();
+    return overlap(a->k, b->k, na, nb) || overlap(a->k, b->v, na, nb) || overlap(a->v, b->k, na, nb) || overlap(a->v, b->v, na, nb);
+}
+
 // Status of a scratch request that came back empty: out of memory, or a capture that cannot allocate.
 int32_t no_scratch(focr_hip_ctx* ctx) { return ctx->captures() ? FOCR_HIP_E_STATE : FOCR_HIP_E_OOM; }
 
@@ -211,8 +222,9 @@ int32_t focr_hip_paged_create(focr_hip_ctx* ctx, size_t n_pages, size_t page_siz
         c->dtype = dtype;
         c->k = k_pool;
         c->v = v_pool;
+        const size_t bytes = n_pages * c->page_bytes();
+        if (k_pool && overlap(k_pool, v_pool, bytes, bytes)) return fail(FOCR_HIP_E_ARG, "paged_create: the pools overlap");
         if (!k_pool) {
-            const size_t bytes = n_pages * c->page_bytes();
             FOCR_HIP_TRY(hipMalloc(&c->k, bytes), "hipMalloc paged K");
             hipError_t e = hipMalloc(&c->v, bytes);
             if (e == hipSuccess) e = hipMemsetAsync(c->k, 0, bytes, ctx->stream);
@@ -480,8 +492,8 @@ int32_t focr_hip_beam_reorder_weighted(focr_hip_ctx* ctx, size_t groups, size_t 
         for (size_t i = 0; i < n_caches; ++i) {
             if ((st = cache_ok(who, ctx, caches[i]))) return st;
             for (size_t j = 0; j < i; ++j)
-                if (caches[i]->k == caches[j]->k || caches[i]->v == caches[j]->v)
-                    return fail(FOCR_HIP_E_ARG, fmt("beam_reorder: caches %zu and %zu are the same", j, i));
+                if (overlap(caches[i], caches[j]))
+                    return fail(FOCR_HIP_E_ARG, fmt("beam_reorder: caches %zu and %zu are the same, or their pools overlap", j, i));
             if (caches[i]->page_shift != caches[0]->page_shift)
                 return fail(FOCR_HIP_E_SHAPE, "beam_reorder: caches of different page sizes share no tables");
             if (!weights || !weights[i]) continue;

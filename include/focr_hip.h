@@ -445,7 +445,7 @@ int32_t focr_hip_rswa_regions(const focr_hip_rswa* cache, size_t stream, float**
  * that is none) before anything is written. With check = 0 a length is cut to
  * max_len and a slot on a page that is none is not read or written. */
 /* Pools of the handle's own (zeroed; k_pool and v_pool null) or of the
- * caller's (16-byte aligned device arrays, not freed). dtype FOCR_HIP_DT_F32,
+ * caller's (16-byte aligned device arrays that do not overlap, not freed). dtype FOCR_HIP_DT_F32,
  * _F16 or _BF16; page_size a power of two up to 1024; head_dim 64, 128 or 256;
  * n_pages * n_kv_heads * page_size < 2^32 - 1. */
 int32_t focr_hip_paged_create(focr_hip_ctx* ctx, size_t n_pages, size_t page_size, size_t n_kv_heads,

@@ -325,6 +325,27 @@ def test_refusals(ctx):
                 ctx.empty((0, 256), np.float32), n_heads=4)  # no sequences: nothing to do
 
 
+def test_overlapping_pools_are_refused(ctx):
+    """Keys and values in one memory, and caches of one call that share some: every row would be written twice."""
+    _say("overlapping pools")
+    from franken_ocr_amd.device import DeviceArray
+    from franken_ocr_amd.engine import PagedCache, beam_reorder
+
+    page = 2 * 16 * 64 * 4
+    pool = ctx.empty((20 * page,), np.uint8)
+    at = lambda p: DeviceArray.borrow(ctx, pool.ptr + p * page, (4 * page,), np.uint8)  # noqa: E731
+    for k, v in ((0, 0), (0, 3), (7, 4)):
+        with pytest.raises(_abi.FocrHipError, match="pools overlap"):
+            PagedCache(4, 16, 2, 64, "f32", k=at(k), v=at(v), ctx=ctx)
+    pair = lambda k, v: PagedCache(4, 16, 2, 64, "f32", k=at(k), v=at(v), ctx=ctx)  # noqa: E731
+    a, n, p = pair(0, 4), ctx.to_device(np.zeros(2, np.uint32)), ctx.to_device(np.array([1, 0], np.uint32))
+    t = ctx.to_device(np.array([[0, 1], [2, 3]], np.uint32))
+    for k, v in ((8, 1), (4, 8), (3, 12), (8, 7)):
+        with pytest.raises(_abi.FocrHipError, match="overlap"):
+            beam_reorder(p, 2, caches=[a, pair(k, v)], tables=t, lens=n)
+    beam_reorder(p, 2, caches=[a, pair(8, 12)], tables=t, lens=n)  # end to end
+
+
 def test_scores_without_an_end(ctx):
     """Keys of -inf scores count for nothing; where there are no others, 0 / 0; a NaN key spreads."""
     _say("infinite scores")
