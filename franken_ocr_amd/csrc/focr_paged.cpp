@@ -478,6 +478,8 @@ int32_t focr_hip_beam_reorder_weighted(focr_hip_ctx* ctx, size_t groups, size_t 
         if (history && (!history_len || history_cap == 0 || history_cap > kI32Max))
             return fail(FOCR_HIP_E_ARG, "beam_reorder: a history needs history_len and a history_cap of 1 .. 2^31 - 1");
         if ((n_caches && !caches) || (n_rings && !rings)) return fail(FOCR_HIP_E_ARG, "beam_reorder: null handles");
+        if (tables && !n_caches)
+            return fail(FOCR_HIP_E_ARG, "beam_reorder: tables move with the caches that share them, and none is given");
         const size_t rows = groups * beams;
         int32_t st;
         BeamReorder a{};

@@ -542,7 +542,8 @@ int32_t focr_hip_beam_select(focr_hip_ctx* ctx, const float* logits, size_t ld, 
  *    cursors, whose agreement is the caller's to keep).
  * So the beams of a group may share the pages they have filled and must not
  * share the one in progress. A parent that is not below beams is taken as the
- * slot itself, a group whose lengths differ keeps its tables and pages;
+ * slot itself, a group whose lengths differ keeps its tables and pages; tables
+ * without caches are refused (E_ARG), for their pages in progress would stay;
  * check = 1 reports these (E_SHAPE, E_STATE) before anything is written. */
 int32_t focr_hip_beam_reorder(focr_hip_ctx* ctx, size_t groups, size_t beams, const uint32_t* parents,
                               const uint32_t* tokens, uint32_t* history, size_t history_cap,

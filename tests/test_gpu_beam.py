@@ -464,6 +464,15 @@ def test_search_gathers_and_evicts_by_its_own_beams(ctx):
                 assert np.array_equal(x[dst[r, slots // page], h, slots % page], rows_of[stay, h])
 
 
+def test_reorder_refuses_tables_without_their_caches(ctx):
+    _say("tables without caches")
+    from franken_ocr_amd.engine import beam_reorder
+
+    u = lambda *s: ctx.to_device(np.zeros(s, np.uint32))  # noqa: E731
+    with pytest.raises(_abi.FocrHipError, match="none is given"):
+        beam_reorder(u(2), 2, tables=u(2, 2), lens=u(2))
+
+
 def test_reorder_refuses_weights_that_do_not_fit(ctx):
     _say("refusals of weights")
     from franken_ocr_amd.engine import PagedCache, beam_reorder
