@@ -420,36 +420,36 @@ class PagedCache:
 
     def _heads(self, who: str, q: DeviceArray, out: DeviceArray, n: int, n_heads, ldq, ldo):
         if n_heads is None:
-            wide = self._pitch(q, n, 0)
-            heads = (wide or q.shape[-1]) // self.head_dim
-            if wide % self.head_dim:
+            shape = q.shape
+            wide = shape[1] if len(shape) == 2 and shape[0] >= n else self._width(q, n, 0) or shape[-1]
+            n_heads = wide // self.head_dim
+            if wide % self.head_dim and len(shape) > 1:
                 raise _abi.ContractViolation(_abi.E_SHAPE, f"{who}: q rows of {wide} are no whole heads of {self.head_dim}")
-        else:
-            heads = n_heads
-        row = heads * self.head_dim
-        ldq, ldo = ldq or self._pitch(q, n, row), ldo or self._pitch(out, n, row)
-        self._fits(who, "q", q, n, row, ldq)
-        self._fits(who, "out", out, n, row, ldo)
-        return heads, ldq, ldo
+        row = n_heads * self.head_dim
+        return n_heads, self._stride(who, "q", q, n, row, ldq), self._stride(who, "out", out, n, row, ldo)
 
     @staticmethod
-    def _pitch(a, rows: int, row: int) -> int:
-        """Values from a row of the array to the next: its width where it has that many rows of at least `row`, else
-        `row` (flat arrays, raw pointers)."""
-        if type(a) is DeviceArray and len(a.shape) > 1 and a.shape[0] >= rows:
-            wide = a.shape[1] if len(a.shape) == 2 else math.prod(a.shape[1:])
-            return wide if wide > row else row
-        return row
+    def _width(a, rows: int, row: int) -> int:
+        """Values from a row of the array to the next where it has that many rows of at least `row`, else `row` (flat
+        arrays)."""
+        return max(row, math.prod(a.shape[1:])) if len(a.shape) > 1 and a.shape[0] >= rows else row
 
-    def _kv(self, who: str, k, v, rows: int, ldkv, names=("k", "v")) -> int:
-        row = self.n_kv_heads * self.head_dim
-        if not ldkv:
-            ldkv, ldv = self._pitch(k, rows, row), self._pitch(v, rows, row)
-            if ldkv != ldv:
-                raise _abi.ContractViolation(_abi.E_SHAPE, f"{who}: {names[0]} rows of {ldkv} and {names[1]} rows of {ldv}")
-        self._fits(who, names[0], k, rows, row, ldkv)
-        self._fits(who, names[1], v, rows, row, ldkv)
-        return ldkv
+    def _stride(self, who: str, name: str, a, rows: int, row: int, ld) -> int:
+        """The stride of `rows` rows of `row` values: ld where it is given, else the array's width (of a raw pointer, which
+        is taken on trust, `row`); the array holds them."""
+        if type(a) is not DeviceArray:
+            return ld or row
+        if not ld:
+            shape = a.shape
+            ld = shape[1] if len(shape) == 2 and shape[0] >= rows and shape[1] >= row else self._width(a, rows, row)
+        if rows and a.nbytes < 4 * ((rows - 1) * ld + row):
+            raise _abi.ContractViolation(_abi.E_SHAPE, f"{who}: {name} of shape {a.shape} holds no {rows} rows of {row}")
+        return ld
+
+    @staticmethod
+    def _alike(who: str, ldk: int, ldv: int) -> None:
+        if ldk != ldv:
+            raise _abi.ContractViolation(_abi.E_SHAPE, f"{who}: k rows of {ldk} and v rows of {ldv}")
 
     @staticmethod
     def _fits(who: str, name: str, a, rows: int, wide: int, ld=None, size: int = 4) -> None:
@@ -462,8 +462,10 @@ class PagedCache:
         """Rows k / v [rows, n_kv_heads * head_dim] into slots pos[i] of the
         sequences seq[i] (sequence i without seq); NO_SEQUENCE skips a row."""
         n, wide = tables.shape
-        rows = pos.shape[0]
-        ldkv = self._kv("paged_write", k, v, rows, ldkv)
+        rows, row = pos.shape[0], self.n_kv_heads * self.head_dim
+        ldv = self._stride("paged_write", "v", v, rows, row, ldkv)
+        ldkv = self._stride("paged_write", "k", k, rows, row, ldkv)
+        self._alike("paged_write", ldkv, ldv)
         self._fits("paged_write", "seq", seq, rows, 1)
         _abi.call("focr_hip_paged_write", self.ctx.handle, self._h, _p(k), _p(v), ldkv, rows, _p(seq), _p(pos),
                   _p(tables), n, wide, 1 if check else 0)
@@ -492,9 +494,14 @@ class PagedCache:
         over lens[s] + 1 keys; with advance the lengths are counted up."""
         n, wide = self._rows("paged_step", tables, lens)
         heads, ldq, ldo = self._heads("paged_step", q, out, n, n_heads, ldq, ldo)
-        ldkv = self._kv("paged_step", k_steps, v_steps, n, ldkv, ("k_steps", "v_steps"))
-        self._fits("paged_step", "prefix", prefix, n, 1)
-        ldw = self._weights("paged_step", weights, n)
+        row = self.n_kv_heads * self.head_dim
+        ldv = self._stride("paged_step", "v_steps", v_steps, n, row, ldkv)
+        ldkv = self._stride("paged_step", "k_steps", k_steps, n, row, ldkv)
+        if ldkv != ldv:
+            self._alike("paged_step", ldkv, ldv)
+        if prefix is not None:
+            self._fits("paged_step", "prefix", prefix, n, 1)
+        ldw = 0 if weights is None else self._weights("paged_step", weights, n)
         _abi.call("focr_hip_paged_step", self.ctx.handle, self._h, _p(q), ldq, heads, _p(k_steps), _p(v_steps),
                   ldkv, _p(tables), n, wide, _p(lens), wide * self.page_size if max_len is None else int(max_len),
                   _p(prefix), int(window), float(scale), _p(out), ldo, _p(weights), ldw, 1 if advance else 0,

@@ -90,7 +90,7 @@ def test_row_strides_are_the_arrays_widths(monkeypatch, shapes, n_heads, want):
 
 @pytest.mark.parametrize("shapes,text", [
     (((4, 250), (4, 128), (4, 128), (4, 256)), "no whole heads"),
-    (((4, 256), (4, 128), (4, 130), (4, 256)), "k_steps rows of 128 and v_steps rows of 130"),
+    (((4, 256), (4, 128), (4, 130), (4, 256)), "k rows of 128 and v rows of 130"),
 ])
 def test_step_refuses_rows_of_no_one_width(shapes, text):
     from franken_ocr_amd import _abi
