@@ -463,11 +463,10 @@ class PagedCache:
         sequences seq[i] (sequence i without seq); NO_SEQUENCE skips a row."""
         n, wide = tables.shape
         rows, row = pos.shape[0], self.n_kv_heads * self.head_dim
-        ldv = self._stride("paged_write", "v", v, rows, row, ldkv)
-        ldkv = self._stride("paged_write", "k", k, rows, row, ldkv)
-        self._alike("paged_write", ldkv, ldv)
+        ldk = self._stride("paged_write", "k", k, rows, row, ldkv)
+        self._alike("paged_write", ldk, self._stride("paged_write", "v", v, rows, row, ldkv))
         self._fits("paged_write", "seq", seq, rows, 1)
-        _abi.call("focr_hip_paged_write", self.ctx.handle, self._h, _p(k), _p(v), ldkv, rows, _p(seq), _p(pos),
+        _abi.call("focr_hip_paged_write", self.ctx.handle, self._h, _p(k), _p(v), ldk, rows, _p(seq), _p(pos),
                   _p(tables), n, wide, 1 if check else 0)
 
     def attention(self, q: DeviceArray, tables: DeviceArray, lens: DeviceArray, out: DeviceArray,
@@ -495,15 +494,15 @@ class PagedCache:
         n, wide = self._rows("paged_step", tables, lens)
         heads, ldq, ldo = self._heads("paged_step", q, out, n, n_heads, ldq, ldo)
         row = self.n_kv_heads * self.head_dim
+        ldk = self._stride("paged_step", "k_steps", k_steps, n, row, ldkv)
         ldv = self._stride("paged_step", "v_steps", v_steps, n, row, ldkv)
-        ldkv = self._stride("paged_step", "k_steps", k_steps, n, row, ldkv)
-        if ldkv != ldv:
-            self._alike("paged_step", ldkv, ldv)
+        if ldk != ldv:
+            self._alike("paged_step", ldk, ldv)
         if prefix is not None:
             self._fits("paged_step", "prefix", prefix, n, 1)
         ldw = 0 if weights is None else self._weights("paged_step", weights, n)
         _abi.call("focr_hip_paged_step", self.ctx.handle, self._h, _p(q), ldq, heads, _p(k_steps), _p(v_steps),
-                  ldkv, _p(tables), n, wide, _p(lens), wide * self.page_size if max_len is None else int(max_len),
+                  ldk, _p(tables), n, wide, _p(lens), wide * self.page_size if max_len is None else int(max_len),
                   _p(prefix), int(window), float(scale), _p(out), ldo, _p(weights), ldw, 1 if advance else 0,
                   1 if check else 0)
 
