@@ -200,6 +200,29 @@ def test_attention_and_step_against_64_bits(ctx, case, step):
     assert np.array_equal(again.numpy(), got)
 
 
+MANY_SPLITS = [  # more than 64 splits of a row, whose joins have 1024 threads
+    ("bf16", 4, 4, 64, 16, [5000, 100, 0], 0, 0),
+    ("f32", 3, 1, 64, 64, [4800, NONE, 4799], 0, 0),
+    ("f16", 2, 1, 256, 32, [5000, 64], 0, 0),
+    ("bf16", 2, 2, 256, 128, [6001], 5000, 100),
+]
+EVERY_KERNEL = [(dtype, 2 * group, 2, dim, 8, [70, 0, NONE, 17], 0, 0)
+                for dtype in ("f32", "f16", "bf16") for dim in (64, 128, 256) for group in (1, 2, 3)]
+
+
+@pytest.mark.parametrize("step", [False, True])
+@pytest.mark.parametrize("case", range(len(MANY_SPLITS)))
+def test_joins_of_many_splits_against_64_bits(ctx, monkeypatch, case, step):
+    monkeypatch.setitem(globals(), "CASES", MANY_SPLITS)
+    test_attention_and_step_against_64_bits(ctx, case, step)
+
+
+@pytest.mark.parametrize("case", range(len(EVERY_KERNEL)))
+def test_steps_of_every_type_width_and_group_against_64_bits(ctx, monkeypatch, case):
+    monkeypatch.setitem(globals(), "CASES", EVERY_KERNEL)
+    test_attention_and_step_against_64_bits(ctx, case, True)
+
+
 def test_write_rows_of_several_sequences(ctx):
     _say("write")
     rng = np.random.default_rng(7)
@@ -675,6 +698,18 @@ def test_evict_keeps_the_heaviest(ctx, dtype, kv, dim, page, lens, budget, sinks
     cache.evict(ctx.to_device(host.tables), dl, dw, budget, ctx.to_device(dst), dl, dst_w, sinks=sinks, recent=recent,
                 max_len=longest)
     host.same_pools()
+
+
+@pytest.mark.parametrize("dtype,kv,dim,page,lens,budget,sinks,recent", [
+    ("bf16", 2, 64, 128, [12000, 9000, 8193, 5, NONE], 4000, 4, 128),                   # a row in one tile of 16384 slots
+    ("f16", 1, 64, 64, [16384, 16383], 12300, 0, 1),                                    # ties at the threshold: zeros
+    ("bf16", 2, 64, 128, [33000, 17000, 16385, 16384] + [40 + s for s in range(61)], 25000, 1, 300),  # 130 rows: tile by tile
+    ("f16", 3, 64, 128, [100] * 50 + [40001], 29000, 7, 0),                             # the same, ties across its tiles
+    ("bf16", 2, 64, 128, [40001, 300, 0, NONE, 16385], 29000, 7, 0),                    # few rows: a block to a tile
+    ("f32", 2, 256, 16, [500, 90], 100, 3, 20),                                         # rows of 1 KB
+])
+def test_evict_of_every_selection(ctx, dtype, kv, dim, page, lens, budget, sinks, recent):
+    test_evict_keeps_the_heaviest(ctx, dtype, kv, dim, page, lens, budget, sinks, recent)
 
 
 # ---- graphs, streams, contexts --------------------------------------------------------
