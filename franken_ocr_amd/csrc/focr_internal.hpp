@@ -758,13 +758,13 @@ struct PagedEvict {
     uint32_t* kept;  // [n_seqs][n_kv_heads][budget]
     uint32_t* hist;  // paged_evict_hist_words() of workspace, null for 0
 };
-// Rows of more than a block's tile are selected by a block to a tile while
-// there are fewer of them than CUs, else by a block to a row; these words are
-// the first way's picks and histograms.
+// Rows of more than 16384 slots are selected by a block to a tile of 8192 while
+// there are at most half as many of them as CUs, all others by a block to a row;
+// these words are the first way's picks and histograms (0: the other way).
 size_t paged_evict_hist_words(size_t rows, uint32_t max_len, int cu_count);
 hipError_t launch_paged_evict(hipStream_t s, const focr_hip_paged* c, const PagedEvict& a, focr_hip_ctx* ctx);
-// Checks for calls that ask for them: err[0] = 0 where all is well, else
-// (row << 8 | code) + 1 of the first fault.
+// Checks for calls that ask for them: err[0], all ones before, becomes the least
+// row << 8 | code of the faults found, and stays all ones where there is none.
 enum PagedFault : int { kFaultLen = 1, kFaultPage = 2, kFaultSeq = 3, kFaultDstPage = 4, kFaultDstShared = 5,
                         kFaultParent = 6, kFaultGroupLen = 7, kFaultTail = 8, kFaultHistory = 9 };
 hipError_t launch_paged_check(hipStream_t s, const focr_hip_paged* c, const PagedTables& t, uint32_t add,

@@ -128,8 +128,9 @@ __device__ __forceinline__ int ban_chunk(const BeamSelect& a, int row, uint32_t 
 // be among them. They are few; they are listed and each counts the greater
 // ones. Where the list does not hold them (long runs of equal logits), the
 // maximum is taken W times instead. 64 rows of 129280 logits for W = 8 take 16
-// us (33 MB): issue of vector instructions, some 700 a wave, the sixteen f64
-// exponentials nearly half of them. Taking the maximum W times took 36 us.
+// us (33 MB) with the ban found beforehand: issue of vector instructions, 595 a
+// wave (a tenth of the rows done), the sixteen f64 exponentials nearly half of
+// them. Taking the maximum W times took 36 us.
 __global__ __launch_bounds__(kThreads) void beam_scan_kernel(BeamSelect a, Parts q) {
     __shared__ float s_max[kWaves];
     __shared__ double s_sum[kWaves];
@@ -541,7 +542,9 @@ struct Gathered {
     uint32_t pieces;  // blocks to a head's row
 };
 
-// Grid (head x piece, group, cache): a thread a key of every slot.
+// Grid (head x piece, group, cache): a thread a key of every slot. Bound by HBM:
+// eight groups of eight beams, 12 layers of 10 key heads and 1151 keys, 65 MB
+// read and written, take 20 us behind the reorder's 63.
 template <int WB>
 __global__ __launch_bounds__(256) void beam_weights_kernel(BeamReorder a, Gathered w) {
     __shared__ uint32_t s_parent[WB];

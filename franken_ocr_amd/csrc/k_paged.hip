@@ -1259,10 +1259,19 @@ void attend(hipStream_t s, const focr_hip_paged* c, const PagedAttend& a) {
     const PoolGeom g = geom_of(c);
     const int kv = static_cast<int>(c->n_kv_heads);
     const auto grid = [&](int gt) { return dim3(a.nsplit, kv * ((a.group + gt - 1) / gt), a.t.n_seqs); };
-    // By query heads to a key head, 128 sequences of up to 16384 keys on 2 key
-    // heads, VALU kernel / matrix cores: bf16 128 wide, one 214 / 223 us, two
-    // 223 / 225, three 248 / 227, four 253 / 228; 64 wide 112 / 132, 117 / 133,
-    // 133 / 135, 136 / 135; f32 64 wide, 64 sequences, two 122 / 136, four 142 / 138.
+    // By query heads to a key head (one, two, three, four), VALU kernel / matrix
+    // cores, us; ragged sequences of up to 16384 keys on 2 key heads, 560 MB in all:
+    //   bf16  64 wide  106/108  109/111  115/113  136/115
+    //   bf16 128 wide  109/113  114/115  119/117  131/119
+    //   bf16 256 wide  113/133  119/136  125/139  135/142
+    //   f16   64 wide  106/108  109/111  114/114  131/115
+    //   f16  128 wide  109/114  114/117  119/119  124/120
+    //   f16  256 wide  113/119  118/122  125/124  134/126
+    //   f32   64 wide  106/112  109/113  112/115  116/117
+    //   f32  128 wide  110/117  113/119  116/121  121/122
+    //   f32  256 wide  107/140  112/142  116/143  121/146
+    // One rule for all of them: three heads in f32, and three and four in bf16
+    // and f32 at 256 wide, are the faster on the VALU by what stands here.
     if (a.group > 2)
         FOCR_LAUNCH((paged_attend_mfma_kernel<T, D>), grid(16), dim3(256), 0, s, g, a);
     else if (a.group == 2)
@@ -1308,7 +1317,11 @@ hipError_t launch_paged_attend(hipStream_t s, const focr_hip_paged* c, const Pag
     ProfScope ps(ctx, "paged_join");
     const uint32_t chunks = a.weights ? static_cast<uint32_t>((a.score_ld + kWeightKeys - 1) / kWeightKeys) : 0;
     const dim3 grid(kv * (a.group + chunks), a.t.n_seqs);
-    // 1024 threads where a row has many splits to join (64 rows of 256 splits: 10 -> 7.5 us)
+    // 1024 threads where a row has many splits to join (64 rows of 256 splits: 10
+    // -> 7.5 us). Whole calls at 256 / 1024 threads, us: 2 x 16384 keys, 32 heads
+    // on 8, 32.7 / 32.2, 2 x 131071 171 / 169, 64 x 65536, 16 on 2, 233 / 234;
+    // with weights, whose blocks then have 512 keys for 1024 threads, 36.1 / 35.5,
+    // 204 / 216, 352 / 394.
     const bool many = a.nsplit > 64;
     if (c->head_dim == 64)
         many ? launch_join<64, 1024>(s, grid, a, kv) : launch_join<64, 256>(s, grid, a, kv);

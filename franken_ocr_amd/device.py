@@ -149,8 +149,11 @@ class DeviceArray:
     @classmethod
     def borrow(cls, ctx: Context, ptr: int, shape, dtype, owner=None) -> "DeviceArray":
         """Device memory that something else owns, as a DeviceArray (it frees
-        nothing; `owner`, if given, is kept alive). Work of other streams on
-        it is the caller's to order."""
+        nothing; `owner`, if given, is kept alive). The context's stream waits
+        for no other, nor they for it: work on the memory from elsewhere is the
+        caller's to order, by waiting for the device or by events between that
+        stream and `ctx.stream()` (torch: ExternalStream(ctx.stream()) and its
+        wait_stream, each way)."""
         a = cls.adopt(ctx, C.c_void_p(int(ptr)), shape, dtype)
         a._borrowed = owner if owner is not None else True
         return a

@@ -443,7 +443,9 @@ int32_t focr_hip_rswa_regions(const focr_hip_rswa* cache, size_t stream, float**
  * check = 1 waits for the stream, looks at what the tables and lengths hold
  * and returns E_STATE (a length past max_len or the tables) or E_SHAPE (a page
  * that is none) before anything is written. With check = 0 a length is cut to
- * max_len and a slot on a page that is none is not read or written. */
+ * max_len and a slot on a page that is none is not read or written: its score
+ * is -inf, so a sequence that sees such slots alone has 0 / 0, NaN, as output
+ * and added to its weights. */
 /* Pools of the handle's own (zeroed; k_pool and v_pool null) or of the
  * caller's (16-byte aligned device arrays that do not overlap, not freed). dtype FOCR_HIP_DT_F32,
  * _F16 or _BF16; page_size a power of two up to 1024; head_dim 64, 128 or 256;
@@ -468,8 +470,10 @@ int32_t focr_hip_paged_write(focr_hip_ctx* ctx, focr_hip_paged* cache, const flo
  * first min(prefix[s], n) (prefix null: none) and the last `window` — with the
  * prompt's length as prefix and a window of 128 what the R-SWA ring sees. out
  * [n_seqs][n_heads * head_dim] (rows ldo apart) = softmax(scale q.k) v, scale
- * not negative and 0 meaning 1 / sqrt(head_dim); zeros where there is no key. The sums are f32,
- * and the same call gives the same bits. weights (nullable)
+ * not negative and 0 meaning 1 / sqrt(head_dim); zeros where there is no key.
+ * The sums are f32, divided by the probabilities' at the end (a value counts up
+ * to 2^8 times in them, so values times keys are to stay below 2^120), and the
+ * same call gives the same bits. weights (nullable)
  * [n_seqs][n_kv_heads][ldw], ldw >= max_len: every key that is seen has the
  * probabilities of its key head's query heads added. */
 int32_t focr_hip_paged_attention(focr_hip_ctx* ctx, const focr_hip_paged* cache, const float* q, size_t ldq,
@@ -518,7 +522,9 @@ int32_t focr_hip_paged_evict(focr_hip_ctx* ctx, focr_hip_paged* cache, const uin
  * no candidates but part of the sum. A beam with done[row] != 0 (nullable) has
  * one candidate, eos_token_id at its score. The first `beams` of the order
  * (score descending, beam ascending, logit descending, token ascending) give
- * parents (the beam within its group), tokens, new_scores (may be scores) and
+ * parents (the beam within its group), tokens, new_scores (may be scores; the
+ * f64 score rounded to f32, so over many steps the order of beams is good to the
+ * f32 roundings that their scores have gathered, half a unit of place a step) and
  * new_done (nullable, may be done: the parent's, or token == eos_token_id).
  * Slots left over take themselves, eos_token_id, -inf and done. check = 1
  * reports a history_len over history_cap (E_SHAPE). */

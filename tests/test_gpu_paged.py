@@ -265,6 +265,25 @@ def test_bad_pages_are_neither_read_nor_written(ctx):
         assert np.allclose(got[0].reshape(2, 64)[h], (p / p.sum()) @ v[:, h], rtol=0, atol=1e-4)
 
 
+@pytest.mark.parametrize("heads", [2, 8])
+def test_a_sequence_on_pages_that_are_none(ctx, heads):
+    """Without check: 0 / 0 where no slot that is seen has a page, the other sequences as they are."""
+    _say(f"pages of nobody, {heads} heads")
+    rng = np.random.default_rng(19)
+    host = Host(rng, ctx, [30, 20, 40], 16, 2, 64, "bf16")
+    bad = host.tables.copy()
+    bad[1] = NONE
+    q = rng.standard_normal((3, heads, 64)).astype(np.float32)
+    dout, dw = ctx.empty((3, heads * 64), np.float32), ctx.to_device(np.zeros((3, 2, 48), np.float32))
+    host.cache.attention(ctx.to_device(q.reshape(3, -1)), ctx.to_device(bad), host.dl, dout, weights=dw)
+    got, gw = dout.numpy().reshape(3, heads, 64), dw.numpy()
+    assert np.all(np.isnan(got[1])) and np.all(np.isnan(gw[1, :, :20])) and np.all(gw[1, :, 20:] == 0)
+    for s in (0, 2):
+        out, tol, keys, w, wt = _attend(host, s, q[s], host.lens[s], 0, 0, 1.0 / np.sqrt(np.float32(64)))
+        assert np.all(np.abs(got[s] - out) <= tol)
+        assert np.all(np.abs(gw[s][:, keys] - w) <= wt + U * (1 + w))
+
+
 @pytest.mark.parametrize("what", ["len", "page", "full", "dst page", "dst shared", "dst read", "seq", "pos"])
 def test_check_reports_before_anything_is_written(ctx, what):
     _say(f"check: {what}")
