@@ -352,12 +352,14 @@ __global__ __launch_bounds__(256, GT == 1 ? 4 : 3) void paged_attend_kernel(Pool
 // the second f16 term is what the first leaves, times 2^12, with sums of its
 // own: for values from 2^-14 on, the first is a normal number and the second
 // holds the rest to 2^-23 of the value (unscaled, it would be subnormal below
-// 2^-2). Values below 2^-14 have no such terms, and infinities have none in
-// either type (an infinite K times a term that is zero is NaN): a wave that
-// meets a smaller coordinate of q or probability (2^-28 of the reference's), or
-// whose sums come out not finite, does its keys in f32 products instead. In f16
-// that costs where scores are far apart: 120 us as below, 144 to 153 where most
-// waves meet such a probability, 134 with the f32 products alone.
+// 2^-2). Values below 2^-14 have no such terms: 16 keys with a smaller
+// probability (2^-28 of the reference's) take f32 products into the same sums,
+// a row of q with a smaller coordinate takes them throughout. Infinities have no
+// terms in either type (an infinite K times a term that is zero is NaN): a wave
+// whose sums come out not finite does its keys again in f32 products. Where the
+// scores of most keys are that far apart, f16 takes 126 us for the 120 below
+// (128 wide 245 for 232, 256 wide 88 for 76, 32 sequences), f32 products for
+// all 134; doing all of a wave's keys again at the first such probability 154.
 // The running maximum is moved only where a score is well past it (any
 // reference gives the same quotient, and f32 holds the sums), so the usual
 // tile needs nothing from other lanes.
@@ -483,7 +485,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_attend_mfma_kerne
             return *reinterpret_cast<const u4*>(p);
         }
     };
-    // false where a value has no terms: the sums are of no use then
+    // false, and nothing done, where q has no terms
     const auto run = [&](auto f32_products) -> bool {
         constexpr bool EXACT = decltype(f32_products)::value;
         constexpr bool APART = !EXACT && TT::kApart != 1.0f;
@@ -639,10 +641,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_attend_mfma_kerne
                 l += p[i];
                 least = min(least, size_order(p[i]));
             }
-            if constexpr (APART) {
-                if (__any(least < size_order(TT::kLeast))) return false;
-            }
-            if constexpr (EXACT) {
+            const bool few = APART && __any(least < size_order(TT::kLeast));
+            if (EXACT || few) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -652,7 +652,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_attend_mfma_kerne
 #pragma unroll
                         for (int j = 0; j < VE; ++j) acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[i], f[j], acc[c][j], 0, 0, 0);
                     }
-            } else {
+                // and zeros for the terms: as the other branch these products took 46 registers more at D = 256
+                if constexpr (APART) p[0] = p[1] = p[2] = p[3] = 0.0f;
+            }
+            if constexpr (!EXACT) {
                 uint32_t w0[TT::N], w1[TT::N];
                 TT::split2(p[0], p[1], w0);
                 TT::split2(p[2], p[3], w1);
