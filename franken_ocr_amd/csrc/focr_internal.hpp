@@ -236,7 +236,7 @@ struct focr_hip_rswa {
 // [page_size][head_dim] each, and their geometry. Page tables and lengths are
 // the caller's device arrays, given with every call.
 struct focr_hip_paged {
-    focr_hip_ctx* ctx = nullptr;
+    int device = 0;  // not the context, which the pools may outlive
     size_t n_pages = 0, n_kv_heads = 0, head_dim = 0;
     int page_shift = 0;  // page_size = 1 << page_shift
     int32_t dtype = 0;   // FOCR_HIP_DT_F32 / F16 / BF16

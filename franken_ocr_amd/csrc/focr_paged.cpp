@@ -64,8 +64,8 @@ int32_t no_scratch(focr_hip_ctx* ctx) { return ctx->captures() ? FOCR_HIP_E_STAT
 
 int32_t cache_ok(const char* who, const focr_hip_ctx* ctx, const focr_hip_paged* c) {
     if (!c) return fail(FOCR_HIP_E_BAD_HANDLE, fmt("%s: null paged cache", who));
-    if (c->ctx->device != ctx->device)
-        return fail(FOCR_HIP_E_ARG, fmt("%s: the cache is on device %d, the context on %d", who, c->ctx->device, ctx->device));
+    if (c->device != ctx->device)
+        return fail(FOCR_HIP_E_ARG, fmt("%s: the cache is on device %d, the context on %d", who, c->device, ctx->device));
     return FOCR_HIP_OK;
 }
 
@@ -214,7 +214,7 @@ int32_t focr_hip_paged_create(focr_hip_ctx* ctx, size_t n_pages, size_t page_siz
         if (!aligned16(k_pool) || !aligned16(v_pool))
             return fail(FOCR_HIP_E_ARG, "paged_create: the pools must be 16-byte aligned");
         std::unique_ptr<focr_hip_paged> c(new focr_hip_paged());
-        c->ctx = ctx;
+        c->device = ctx->device;
         c->n_pages = n_pages;
         c->n_kv_heads = n_kv_heads;
         c->head_dim = head_dim;
@@ -245,8 +245,8 @@ int32_t focr_hip_paged_create(focr_hip_ctx* ctx, size_t n_pages, size_t page_siz
 int32_t focr_hip_paged_free(focr_hip_paged* c) {
     if (!c) return FOCR_HIP_OK;
     if (c->owned) {
-        hipSetDevice(c->ctx->device);
-        hipStreamSynchronize(c->ctx->stream);
+        hipSetDevice(c->device);
+        hipDeviceSynchronize();  // calls of any context may be using them
         hipFree(c->k);
         hipFree(c->v);
     }

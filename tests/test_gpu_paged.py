@@ -808,6 +808,31 @@ def test_captured_step_replays_while_lengths_grow(ctx):
         _capture(c, lambda: caches[0].step(q[0], k[0], k[0], dt, lens[0], outs[0], check=True))
 
 
+def test_a_cache_outlives_its_context(ctx):
+    """A cache made with a context that is gone by now: used with another, and freed."""
+    _say("cache of a closed context")
+    from franken_ocr_amd.device import Context
+    from franken_ocr_amd.engine import PagedCache
+
+    rng = np.random.default_rng(23)
+    c = Context(0)
+    cache = PagedCache(6, 16, 1, 64, "f32", ctx=c)
+    c.close()
+    cache.ctx = ctx
+    k, v = (rng.standard_normal((40, 64)).astype(np.float32) for _ in "kv")
+    q = rng.standard_normal((1, 64)).astype(np.float32)
+    t, n, out = ctx.to_device(np.array([[4, 1, 5]], np.uint32)), ctx.to_device(np.array([40], np.uint32)), ctx.empty((1, 64), np.float32)
+    cache.write(ctx.to_device(k), ctx.to_device(v), ctx.to_device(np.arange(40, dtype=np.uint32)), t,
+                seq=ctx.to_device(np.zeros(40, np.uint32)), check=True)
+    cache.attention(ctx.to_device(q), t, n, out, check=True)
+    sc = k.astype(np.float64) @ q[0] / 8
+    p = np.exp(sc - sc.max())
+    p /= p.sum()
+    tol = (p @ np.abs(v)) * 2 * (72 * U * (np.abs(k) @ np.abs(q[0])).max() / 8 + 2.0 ** -22 + 104 * U)
+    assert np.all(np.abs(out.numpy()[0] - p @ v) <= tol)
+    cache.free()
+
+
 def test_two_contexts_at_once(ctx):
     """Calls of two contexts on caches of their own, issued in turn without waiting."""
     _say("two contexts")
