@@ -474,8 +474,8 @@ int32_t focr_hip_paged_write(focr_hip_ctx* ctx, focr_hip_paged* cache, const flo
  * The sums are f32, divided by the probabilities' at the end (a value counts up
  * to 2^8 times in them, so values times keys are to stay below 2^120), and the
  * same call gives the same bits. weights (nullable)
- * [n_seqs][n_kv_heads][ldw], ldw >= max_len: every key that is seen has the
- * probabilities of its key head's query heads added. */
+ * [n_seqs][n_kv_heads][ldw], ldw >= max_len, zeros at first: every key that is
+ * seen has the probabilities of its key head's query heads added. */
 int32_t focr_hip_paged_attention(focr_hip_ctx* ctx, const focr_hip_paged* cache, const float* q, size_t ldq,
                                  size_t n_heads, const uint32_t* tables, size_t n_seqs, size_t max_pages,
                                  const uint32_t* lens, size_t max_len, const uint32_t* prefix,
@@ -500,8 +500,9 @@ int32_t focr_hip_paged_step(focr_hip_ctx* ctx, focr_hip_paged* cache, const floa
  * pages of dst_tables [n_seqs][dst_max_pages], which no sequence of the call
  * may read and no two share (source pages may be shared, so nothing moves
  * within them). dst_lens [n_seqs] = min(n, budget); dst_weights
- * [n_seqs][n_kv_heads][dst_ldw] the weights of the slots that stay; kept
- * (nullable) [n_seqs][n_kv_heads][budget] their slots. With several layers
+ * [n_seqs][n_kv_heads][dst_ldw] the weights of the slots that stay (those behind
+ * them are left: zeros, if later keys are to gather there); kept (nullable)
+ * [n_seqs][n_kv_heads][budget] their slots. With several layers
  * each has weights, so evicts, of its own, and the new lengths agree; dst_lens
  * may be lens in the last of the calls that read it. */
 int32_t focr_hip_paged_evict(focr_hip_ctx* ctx, focr_hip_paged* cache, const uint32_t* tables, size_t n_seqs,
